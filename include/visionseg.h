@@ -275,6 +275,55 @@ VS_API int vs_mx_quantize(const void* x, void* q, void* scales, int rows, int K,
 VS_API int vs_row_quantize_fp8(const void* x, void* q, float* scale, int rows, int K, void* stream);
 VS_API int vs_gelu_row_quantize_fp8(const void* h, void* y, void* q, float* scale, int rows, int K, void* stream);
 
+/* ---- 8-bit activation checkpoints (csrc/act8.h, act8.hip, act8_norm.hip, act8_wgrad.hip) ----
+ * What the backward pass needs of an activation, kept in one byte an element.  A row of
+ * `features` C is cut into blocks of 32 (the last one shorter where 32 does not divide C); a
+ * block with the largest magnitude a keeps e = the smallest integer >= -126 with a <= 127 * 2^e
+ * and q = round_half_even(x * 2^-e):
+ *   q      int8  [rows, P]      P = C rounded up to a multiple of 32, zeros behind C; 8-B aligned
+ *   scale  uint8 [rows, P / 32] e + 127 (1..248), or 255: the block held a magnitude above
+ *                               127 * 2^121, an infinity or a NaN (q 0) and stands for NaN
+ * It stands for q * 2^e, which bf16 holds exactly.  Rows and features may be 0 (nothing is done)
+ * and features need not be a multiple of anything; data pointers only need their element's
+ * alignment. */
+/* x [rows, features] (dtype; row stride ld_x elements, unit feature stride) -> q, scale. */
+VS_API int vs_act8_pack(int dtype, const void* x, long long ld_x, void* q, void* scale, long long rows, int features,
+                        void* stream);
+/* q, scale -> y [rows, features] (dtype, contiguous): the values. */
+VS_API int vs_act8_unpack(int dtype, const void* q, const void* scale, void* y, long long rows, int features,
+                          void* stream);
+/* y = gelu(x) (exact: x Phi(x)) and the checkpoint of x (q and scale NULL: none); contiguous. */
+VS_API int vs_act8_gelu_forward(int dtype, const void* x, void* y, void* q, void* scale, long long rows, int features,
+                                void* stream);
+/* gx = gy * gelu'(h), h the checkpoint's values; y (may be NULL) = gelu(h) again, the input of
+ * the Linear behind the GELU, for that Linear's weight gradient. */
+VS_API int vs_act8_gelu_backward(int dtype, const void* gy, const void* q, const void* scale, void* gx, void* y,
+                                 long long rows, int features, void* stream);
+/* LayerNorm over the features (<= 8192) of x, or -- r and s not NULL -- of s = x + r, rounded to
+ * dtype and written: y = (x - mean) * rstd * w + b, mean / rstd f32 [rows], and the checkpoint
+ * of the normalised tensor (q and scale NULL: none).  y_rows int32 [rows] (may be NULL): the
+ * row of y [y_count, features] that row i goes to (outside it: nowhere). */
+VS_API int vs_act8_layer_norm_forward(int dtype, const void* x, const void* r, const void* w, const void* b, void* s,
+                                      void* y, void* q, void* scale, float* mean, float* rstd, long long rows,
+                                      int features, float eps, const int* y_rows, long long y_count, void* stream);
+/* Its backward at the checkpointed rows: gx (+= gs, the gradient of s, where gs is not NULL),
+ * gw / gb [features] (dtype, overwritten; 0 where rows is 0).  gy_rows: as y_rows, for gy
+ * [gy_count, features] (outside it: zeros).  Deterministic. */
+VS_API long long vs_act8_layer_norm_backward_workspace_bytes(long long rows, int features);
+VS_API int vs_act8_layer_norm_backward(int dtype, const void* gy, const void* gs, const void* q, const void* scale,
+                                       const void* w, const float* mean, const float* rstd, void* gx, void* gw,
+                                       void* gb, void* workspace, long long rows, int features, const int* gy_rows,
+                                       long long gy_count, void* stream);
+
+/* dW[o, i] = sum_t gy[t, o] h[t, i] and, db not NULL, db[o] = sum_t gy[t, o] of a Linear with N
+ * outputs and K inputs from its output gradient gy [tokens, N] (dtype; row stride ld_gy, unit
+ * feature stride) and the checkpoint of its input (q 16-B aligned): dw [N, K], db [N] in
+ * out_dtype (overwritten; 0 where tokens is 0).  f32 accumulation; bf16 gy: exact products;
+ * f32 gy: exact products too (three bf16 parts).  K > 0.  Deterministic. */
+VS_API long long vs_act8_wgrad_workspace_bytes(long long tokens, int N, int K);
+VS_API int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long ld_gy, const void* q, const void* scale,
+                         void* dw, void* db, void* workspace, long long tokens, int N, int K, void* stream);
+
 /* ---- a11: mask head -----------------------------------------------------------------
  * logits f32 [B, Q, H*W] = E [B, Q, C] x P[b]^T, with the pixel embedding P
  * channels-last [B, H*W, C] (HF:m2f:2051 einsum 'bqc,bchw->bqhw').  dtype of E and P:

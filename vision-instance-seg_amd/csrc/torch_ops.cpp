@@ -12,9 +12,11 @@
 //
 // Host-only C++ (g++), linked against libvisionseg_hip.so; the kernels live in csrc/*.hip.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -460,6 +462,208 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> self_attn_bwd(const at::Tensor& q
   return {gq, gk, gv};
 }
 
+
+// ---- 8-bit activation checkpoints (q int8 [..., P], scale uint8 [..., P / 32], P = the features
+// rounded up to 32).  The outputs and workspaces are the caller's device's and stream's; the
+// device guard makes a call on tensors of another device than the current one run there.
+int64_t padded_features(int64_t C) { return (C + 31) / 32 * 32; }
+
+void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> ts) {
+  on_device({&a});
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(t->device() == a.device(), "tensors on different devices: ", a.device(), " and ", t->device());
+}
+
+// x as rows of its last dimension: unit feature stride, any row stride
+at::Tensor as_rows(const at::Tensor& x, const char* what) {
+  TORCH_CHECK(x.dim() >= 1, what, " must have at least one dimension");
+  dcode(x);
+  TORCH_CHECK(x.size(-1) <= (1 << 30), what, ": at most 2^30 features");
+  if (x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1)) return x;
+  const int64_t C = x.size(-1);
+  at::Tensor r = x.contiguous().view({C ? x.numel() / C : 0, C});
+  return r;
+}
+
+at::Tensor dense(const at::Tensor& x) { return x.contiguous(); }
+
+at::Tensor new_q(const at::Tensor& x) {
+  auto sz = x.sizes().vec();
+  sz.back() = padded_features(sz.back());
+  return at::empty(sz, x.options().dtype(at::kChar));
+}
+at::Tensor new_scale(const at::Tensor& x) {
+  auto sz = x.sizes().vec();
+  sz.back() = padded_features(sz.back()) / 32;
+  return at::empty(sz, x.options().dtype(at::kByte));
+}
+
+// the checkpoint's tensors against the features it is said to have -> rows
+int64_t check_checkpoint(const at::Tensor& q, const at::Tensor& scale, int64_t features) {
+  same_device(q, {&scale});
+  TORCH_CHECK(q.scalar_type() == at::kChar && scale.scalar_type() == at::kByte,
+              "a checkpoint is q int8 and scale uint8, got ", q.scalar_type(), " and ", scale.scalar_type());
+  TORCH_CHECK(features >= 0 && features <= (1 << 30), "features out of range: ", features);
+  TORCH_CHECK(q.dim() >= 1 && scale.dim() == q.dim() && q.size(-1) == padded_features(features) &&
+                  scale.size(-1) * 32 == q.size(-1) &&
+                  q.sizes().slice(0, q.dim() - 1) == scale.sizes().slice(0, q.dim() - 1),
+              "q ", q.sizes(), " and scale ", scale.sizes(), " are not a checkpoint of ", features, " features");
+  return q.size(-1) ? q.numel() / q.size(-1) : 0;
+}
+
+std::tuple<at::Tensor, at::Tensor> act8_pack(const at::Tensor& x) {
+  on_device({&x});
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor r = as_rows(x, "x");
+  at::Tensor q = new_q(x), scale = new_scale(x);
+  vs_ok(vs_act8_pack(dcode(r), r.data_ptr(), r.stride(0), q.data_ptr(), scale.data_ptr(), r.size(0), (int)r.size(1),
+                     cur_stream(r)),
+        "act8_pack");
+  return {q, scale};
+}
+
+at::Tensor act8_unpack(const at::Tensor& q, const at::Tensor& scale, int64_t features, at::ScalarType dtype) {
+  on_device({&q});
+  const int64_t rows = check_checkpoint(q, scale, features);
+  const c10::DeviceGuard guard(q.device());
+  auto sz = q.sizes().vec();
+  sz.back() = features;
+  at::Tensor qc = dense(q), sc = dense(scale), y = at::empty(sz, q.options().dtype(dtype));
+  vs_ok(vs_act8_unpack(dcode(y), qc.data_ptr(), sc.data_ptr(), y.data_ptr(), rows, (int)features, cur_stream(qc)),
+        "act8_unpack");
+  return y;
+}
+
+// -> (gelu(x), q, scale); keep false: empty q, scale
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_gelu_fwd(const at::Tensor& x, bool keep) {
+  on_device({&x});
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor xc = dense(x), y = at::empty_like(xc);
+  at::Tensor q = keep ? new_q(xc) : at::empty({0}, xc.options().dtype(at::kChar));
+  at::Tensor scale = keep ? new_scale(xc) : at::empty({0}, xc.options().dtype(at::kByte));
+  const int64_t C = xc.size(-1);
+  TORCH_CHECK(C <= (1 << 30), "x: at most 2^30 features");
+  vs_ok(vs_act8_gelu_forward(dcode(xc), xc.data_ptr(), y.data_ptr(), keep ? q.data_ptr() : nullptr,
+                             keep ? scale.data_ptr() : nullptr, C ? xc.numel() / C : 0, (int)C, cur_stream(xc)),
+        "act8_gelu_fwd");
+  return {y, q, scale};
+}
+
+// -> (gx, gelu(h) or an empty tensor)
+std::tuple<at::Tensor, at::Tensor> act8_gelu_bwd(const at::Tensor& grad_y, const at::Tensor& q, const at::Tensor& scale,
+                                                 bool recompute) {
+  same_device(grad_y, {&q, &scale});
+  TORCH_CHECK(grad_y.dim() >= 1, "grad_y must have at least one dimension");
+  const int64_t C = grad_y.size(-1), rows = check_checkpoint(q, scale, C);
+  TORCH_CHECK(grad_y.sizes().slice(0, grad_y.dim() - 1) == q.sizes().slice(0, q.dim() - 1),
+              "grad_y ", grad_y.sizes(), " does not have the checkpoint's rows ", q.sizes());
+  const c10::DeviceGuard guard(grad_y.device());
+  at::Tensor g = dense(grad_y), qc = dense(q), sc = dense(scale), gx = at::empty_like(g);
+  at::Tensor y = recompute ? at::empty_like(g) : at::empty({0}, g.options());
+  vs_ok(vs_act8_gelu_backward(dcode(g), g.data_ptr(), qc.data_ptr(), sc.data_ptr(), gx.data_ptr(),
+                              recompute ? y.data_ptr() : nullptr, rows, (int)C, cur_stream(g)),
+        "act8_gelu_bwd");
+  return {gx, y};
+}
+
+const int* row_map(const std::optional<at::Tensor>& rows, const at::Tensor& like, int64_t n) {
+  if (!rows.has_value()) return nullptr;
+  same_device(like, {&*rows});
+  TORCH_CHECK(rows->scalar_type() == at::kInt && rows->is_contiguous() && rows->numel() == n,
+              "rows must be contiguous int32, one for each row of x");
+  return rows->data_ptr<int>();
+}
+
+// -> (s, y, q, scale, mean, rstd): s is x without a residual r; rows (int32): y [out_rows, C], row i
+// of x normalised into row rows[i] of y (the others are left unwritten)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> act8_layer_norm_fwd(
+    const at::Tensor& x, const std::optional<at::Tensor>& r, const at::Tensor& weight, const at::Tensor& bias,
+    double eps, const std::optional<at::Tensor>& rows, int64_t out_rows, bool keep) {
+  same_device(x, {&weight, &bias});
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
+  TORCH_CHECK(C >= 1 && C <= 8192, "act8_layer_norm: 1 to 8192 features, got ", C);
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type() && bias.scalar_type() == x.scalar_type() &&
+                  weight.sizes() == at::IntArrayRef({C}) && bias.sizes() == at::IntArrayRef({C}),
+              "weight and bias must be [", C, "] in x's dtype");
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor xc = dense(x), wc = dense(weight), bc = dense(bias), rc, s = xc;
+  if (r.has_value()) {
+    same_device(x, {&*r});
+    TORCH_CHECK(r->sizes() == x.sizes() && r->scalar_type() == x.scalar_type(), "r must be shaped and typed like x");
+    rc = dense(*r);
+    s = at::empty_like(xc);
+  }
+  const int* map = row_map(rows, x, M);
+  TORCH_CHECK(out_rows >= 0, "out_rows must not be negative");
+  at::Tensor y = map ? at::empty({out_rows, C}, xc.options()) : at::empty_like(xc);
+  at::Tensor q = keep ? new_q(xc) : at::empty({0}, xc.options().dtype(at::kChar));
+  at::Tensor scale = keep ? new_scale(xc) : at::empty({0}, xc.options().dtype(at::kByte));
+  at::Tensor mean = at::empty({M}, xc.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  vs_ok(vs_act8_layer_norm_forward(dcode(xc), xc.data_ptr(), r.has_value() ? rc.data_ptr() : nullptr, wc.data_ptr(),
+                                   bc.data_ptr(), r.has_value() ? s.data_ptr() : nullptr, y.data_ptr(),
+                                   keep ? q.data_ptr() : nullptr, keep ? scale.data_ptr() : nullptr,
+                                   mean.data_ptr<float>(), rstd.data_ptr<float>(), M, (int)C, (float)eps, map, out_rows,
+                                   cur_stream(xc)),
+        "act8_layer_norm_fwd");
+  return {s, y, q, scale, mean, rstd};
+}
+
+// -> (gx, gw, gb); grad_s: the gradient of s = x + r, added to gx
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_layer_norm_bwd(
+    const at::Tensor& grad_y, const std::optional<at::Tensor>& grad_s, const at::Tensor& q, const at::Tensor& scale,
+    const at::Tensor& weight, const at::Tensor& mean, const at::Tensor& rstd, const std::optional<at::Tensor>& rows) {
+  same_device(grad_y, {&q, &scale, &weight, &mean, &rstd});
+  TORCH_CHECK(weight.dim() == 1, "weight must be one-dimensional");
+  const int64_t C = weight.size(0), M = check_checkpoint(q, scale, C);
+  TORCH_CHECK(C >= 1 && C <= 8192, "act8_layer_norm: 1 to 8192 features, got ", C);
+  TORCH_CHECK(grad_y.dim() >= 1 && grad_y.size(-1) == C && weight.scalar_type() == grad_y.scalar_type(),
+              "grad_y must have weight's features and dtype");
+  TORCH_CHECK(mean.scalar_type() == at::kFloat && rstd.scalar_type() == at::kFloat && mean.numel() == M &&
+                  rstd.numel() == M && mean.is_contiguous() && rstd.is_contiguous(),
+              "mean / rstd must be contiguous float32, one for each row of the checkpoint");
+  const c10::DeviceGuard guard(grad_y.device());
+  const int* map = row_map(rows, grad_y, M);
+  TORCH_CHECK(map || grad_y.numel() == M * C, "grad_y ", grad_y.sizes(), " does not have the checkpoint's rows");
+  auto sz = q.sizes().vec();
+  sz.back() = C;
+  at::Tensor g = dense(grad_y), qc = dense(q), sc = dense(scale), wc = dense(weight), ds;
+  if (grad_s.has_value()) {
+    same_device(grad_y, {&*grad_s});
+    TORCH_CHECK(grad_s->numel() == M * C && grad_s->scalar_type() == g.scalar_type(),
+                "grad_s must have the checkpoint's rows and grad_y's dtype");
+    ds = dense(*grad_s);
+  }
+  at::Tensor gx = at::empty(sz, g.options()), gw = at::empty_like(wc), gb = at::empty_like(wc);
+  at::Tensor ws = at::empty({vs_act8_layer_norm_backward_workspace_bytes(M, (int)C)}, g.options().dtype(at::kByte));
+  vs_ok(vs_act8_layer_norm_backward(dcode(g), g.data_ptr(), grad_s.has_value() ? ds.data_ptr() : nullptr,
+                                    qc.data_ptr(), sc.data_ptr(), wc.data_ptr(), mean.data_ptr<float>(),
+                                    rstd.data_ptr<float>(), gx.data_ptr(), gw.data_ptr(), gb.data_ptr(),
+                                    ws.data_ptr(), M, (int)C, map, g.numel() / C, cur_stream(g)),
+        "act8_layer_norm_bwd");
+  return {gx, gw, gb};
+}
+
+// -> (dw [N, features], db [N] or an empty tensor) in `dtype`
+std::tuple<at::Tensor, at::Tensor> act8_wgrad(const at::Tensor& grad_y, const at::Tensor& q, const at::Tensor& scale,
+                                              int64_t features, at::ScalarType dtype, bool bias) {
+  same_device(grad_y, {&q, &scale});
+  TORCH_CHECK(features >= 1, "act8_wgrad: at least one feature");
+  const int64_t T = check_checkpoint(q, scale, features);
+  const c10::DeviceGuard guard(grad_y.device());
+  at::Tensor g = as_rows(grad_y, "grad_y"), qc = dense(q), sc = dense(scale);
+  const int64_t N = grad_y.size(-1);
+  TORCH_CHECK(N == 0 || g.size(0) == T, "grad_y has ", g.size(0), " rows, the checkpoint ", T);
+  at::Tensor dw = at::empty({N, features}, g.options().dtype(dtype));
+  at::Tensor db = at::empty({bias ? N : 0}, g.options().dtype(dtype));
+  at::Tensor ws = at::empty({vs_act8_wgrad_workspace_bytes(T, (int)N, (int)features)}, g.options().dtype(at::kByte));
+  vs_ok(vs_act8_wgrad(dcode(g), dcode(dw), g.data_ptr(), g.stride(0), qc.data_ptr(), sc.data_ptr(), dw.data_ptr(),
+                      bias ? db.data_ptr() : nullptr, ws.data_ptr(), T, (int)N, (int)features, cur_stream(g)),
+        "act8_wgrad");
+  return {dw, db};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(visionseg, m) {
@@ -488,6 +692,16 @@ TORCH_LIBRARY(visionseg, m) {
   m.def("self_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor words, int heads, float scale) -> (Tensor, Tensor, Tensor)");
   m.def("self_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor words, Tensor out, Tensor lse, Tensor grad_out, "
         "int heads, float scale) -> (Tensor, Tensor, Tensor)");
+  m.def("act8_pack(Tensor x) -> (Tensor, Tensor)");
+  m.def("act8_unpack(Tensor q, Tensor scale, int features, ScalarType dtype) -> Tensor");
+  m.def("act8_gelu_fwd(Tensor x, bool keep=True) -> (Tensor, Tensor, Tensor)");
+  m.def("act8_gelu_bwd(Tensor grad_y, Tensor q, Tensor scale, bool recompute=False) -> (Tensor, Tensor)");
+  m.def("act8_layer_norm_fwd(Tensor x, Tensor? r, Tensor weight, Tensor bias, float eps, Tensor? rows=None, "
+        "int out_rows=0, bool keep=True) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("act8_layer_norm_bwd(Tensor grad_y, Tensor? grad_s, Tensor q, Tensor scale, Tensor weight, Tensor mean, "
+        "Tensor rstd, Tensor? rows=None) -> (Tensor, Tensor, Tensor)");
+  m.def("act8_wgrad(Tensor grad_y, Tensor q, Tensor scale, int features, ScalarType dtype, bool bias=False) "
+        "-> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(visionseg, CUDA, m) {
@@ -506,4 +720,11 @@ TORCH_LIBRARY_IMPL(visionseg, CUDA, m) {
   m.impl("masked_xattn_bwd", masked_xattn_bwd);
   m.impl("self_attn_fwd", self_attn_fwd);
   m.impl("self_attn_bwd", self_attn_bwd);
+  m.impl("act8_pack", act8_pack);
+  m.impl("act8_unpack", act8_unpack);
+  m.impl("act8_gelu_fwd", act8_gelu_fwd);
+  m.impl("act8_gelu_bwd", act8_gelu_bwd);
+  m.impl("act8_layer_norm_fwd", act8_layer_norm_fwd);
+  m.impl("act8_layer_norm_bwd", act8_layer_norm_bwd);
+  m.impl("act8_wgrad", act8_wgrad);
 }

@@ -125,6 +125,16 @@ SIGNATURES = {
     "vs_transpose_batched": [_c_int, _P, _c_int, _P],
     "vs_token_wgrad": [_c_int, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, _P, _P, ctypes.c_longlong, _c_int,
                        _c_int, _P],
+    "vs_act8_pack": [_c_int, _P, ctypes.c_longlong, _P, _P, ctypes.c_longlong, _c_int, _P],
+    "vs_act8_unpack": [_c_int, _P, _P, _P, ctypes.c_longlong, _c_int, _P],
+    "vs_act8_gelu_forward": [_c_int] + [_P] * 4 + [ctypes.c_longlong, _c_int, _P],
+    "vs_act8_gelu_backward": [_c_int] + [_P] * 5 + [ctypes.c_longlong, _c_int, _P],
+    "vs_act8_layer_norm_forward": [_c_int] + [_P] * 10 + [ctypes.c_longlong, _c_int, _c_float, _P,
+                                                          ctypes.c_longlong, _P],
+    "vs_act8_layer_norm_backward_workspace_bytes": [ctypes.c_longlong, _c_int],
+    "vs_act8_layer_norm_backward": [_c_int] + [_P] * 11 + [ctypes.c_longlong, _c_int, _P, ctypes.c_longlong, _P],
+    "vs_act8_wgrad_workspace_bytes": [ctypes.c_longlong, _c_int, _c_int],
+    "vs_act8_wgrad": [_c_int, _c_int, _P, ctypes.c_longlong] + [_P] * 5 + [ctypes.c_longlong, _c_int, _c_int, _P],
     "vs_conv3x3_forward": [_P, _P, _P, _P] + [_c_int] * 5 + [_P],
     "vs_conv3x3_weight_layouts": [_P, _P, _P, _c_int, _c_int, _P],
     "vs_conv3x3_wgrad_workspace_bytes": [_c_int] * 5,
@@ -144,7 +154,9 @@ RESTYPES = {"vs_last_error": ctypes.c_char_p, "vs_masked_attn_workspace_bytes": 
             "vs_match_cost_factors_workspace_bytes": ctypes.c_longlong,
             "vs_conv3x3_wgrad_workspace_bytes": ctypes.c_longlong,
             "vs_token_wgrad_workspace_bytes": ctypes.c_longlong,
-            "vs_token_wgrad_grouped_workspace_bytes": ctypes.c_longlong}
+            "vs_token_wgrad_grouped_workspace_bytes": ctypes.c_longlong,
+            "vs_act8_layer_norm_backward_workspace_bytes": ctypes.c_longlong,
+            "vs_act8_wgrad_workspace_bytes": ctypes.c_longlong}
 
 _lib = None
 _tops = None

@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
@@ -836,10 +837,13 @@ class TokenLayerNorm(nn.LayerNorm):
             return ops.layer_norm(x, self.weight, self.bias, self.eps)
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
 
-    def forward_windows(self, x, wrows, quant: bool = False):
+    def forward_windows(self, x, wrows, quant: bool = False, act8: bool = False):
         """LN(x) in the window layout of wrows (ops.WindowRows: the Swin partition folded
         into the kernel's stores) -> [wrows.total, C]; quant (bf16, C % 32 == 0): -> (y,
-        (e4m3, e8m0 scales) of y) for an fp8 consumer, (y, None) where the copy cannot be made."""
+        (e4m3, e8m0 scales) of y) for an fp8 consumer, (y, None) where the copy cannot be made;
+        act8: the norm keeps its input in 8 bits (ops.layer_norm_act8)."""
+        if act8 and self._act8_ok(x):
+            return ops.layer_norm_act8(x, self.weight, self.bias, self.eps, wrows=wrows)
         if self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight) \
                 and not torch.is_autocast_enabled():
             if quant and x.dtype == torch.bfloat16 and x.shape[-1] % (8 if quant == "rows" else 32) == 0:
@@ -852,9 +856,15 @@ class TokenLayerNorm(nn.LayerNorm):
         y = ops._to_windows(y.to(_autocast_dtype(y)), wrows)
         return (y, None) if quant else y
 
-    def add_forward_windows(self, x, r, wrows, sink=None, quant: bool = False):
-        """(x + r, LN(x + r) in the window layout of wrows) (+ the MX fp8 copy, see
+    def _act8_ok(self, x) -> bool:
+        return (self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight)
+                and not torch.is_autocast_enabled())
+
+    def add_forward_windows(self, x, r, wrows, sink=None, quant: bool = False, act8: bool = False):
+        """(x + r, LN(x + r) in the window layout of wrows) (+ the MX fp8 copy, act8: see
         forward_windows)."""
+        if act8 and self._act8_ok(x) and r.shape == x.shape and r.dtype == x.dtype:
+            return ops.add_layer_norm_act8(x, r, self.weight, self.bias, self.eps, wrows=wrows)
         if self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight) \
                 and r.shape == x.shape and r.dtype == x.dtype and not torch.is_autocast_enabled():
             if quant and x.dtype == torch.bfloat16 and x.shape[-1] % (8 if quant == "rows" else 32) == 0:
@@ -867,11 +877,13 @@ class TokenLayerNorm(nn.LayerNorm):
         y = ops._to_windows(y.to(_autocast_dtype(y)), wrows)
         return (s, y, None) if quant else (s, y)
 
-    def add_forward(self, x, r, sink=None, quant: bool = False):
+    def add_forward(self, x, r, sink=None, quant: bool = False, act8: bool = False):
         """(x + r, LN(x + r)): the residual add fused into the norm on the HIP kernel
         (ops.add_layer_norm) where the plain norm would run there too.  `sink`: hand x's
         gradient to the armed consumer of x (ops.ResidualSink); `quant`: + the MX fp8 copy of
-        LN(x + r) (see forward_windows)."""
+        LN(x + r), `act8`: x + r kept in 8 bits (see forward_windows)."""
+        if act8 and self._act8_ok(x) and r.shape == x.shape and r.dtype == x.dtype:
+            return ops.add_layer_norm_act8(x, r, self.weight, self.bias, self.eps)
         if self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight) \
                 and r.shape == x.shape and r.dtype == x.dtype and not torch.is_autocast_enabled():
             if quant == "rows" and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
@@ -971,6 +983,117 @@ def linear_relu_tokens(x, w, b, sink=None, act_sink=None):
             and x.dtype in (torch.float32, torch.bfloat16) and N % 8 == 0 and N <= ops.COLSUM_MAX_N and x.is_contiguous()):
         return _LinearReluFn.apply(x, w, b, sink, act_sink)
     return ops.activation(linear_tokens(x, w, b, sink), "relu")
+
+
+# ---------------------------------------------------------------------------------------
+# Linears that keep their input as an 8-bit activation checkpoint (ops.act8_pack)
+# ---------------------------------------------------------------------------------------
+class _LinearAct8Fn(torch.autograd.Function):
+    """x W^T + b keeping x in 8 bits: forward and dX as _LinearFn, dW and db from the checkpoint
+    (ops.act8_wgrad)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        K = x.shape[-1]
+        q, scale = ops.act8_pack(x.reshape(-1, K))
+        ctx.save_for_backward(q, scale, weight)
+        ctx.shape, ctx.has_bias = x.shape, bias is not None
+        T = q.shape[0]
+        ctx.wt = _WT.request(weight) if ctx.needs_input_grad[0] and _dgrad_on_token_gemm(T, weight, x.dtype) else None
+        return _forward_gemm(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        q, scale, weight = ctx.saved_tensors
+        gy2 = gy.reshape(-1, gy.shape[-1]).to(weight.dtype)
+        gx = _dgrad_gemm(gy2, weight, ctx.wt).view(ctx.shape) if ctx.needs_input_grad[0] else None
+        ctx.wt = None
+        want_b = ctx.has_bias and ctx.needs_input_grad[2]
+        gw = gb = None
+        if ctx.needs_input_grad[1]:
+            gw = ops.act8_wgrad(gy2, q, scale, weight.shape[1], weight.dtype, bias=want_b)
+            if want_b:
+                gw, gb = gw
+        elif want_b:
+            gb = gy2.sum(0, dtype=torch.float32).to(weight.dtype)
+        return gx, gw, gb
+
+
+class _MlpAct8Fn(torch.autograd.Function):
+    """fc2(gelu(fc1(x))) (exact GELU) keeping x and the pre-activation in 8 bits: the GELU's
+    output, four times as wide as x and read by fc2's weight gradient alone, is computed again
+    from the pre-activation's checkpoint in the pass that takes the GELU's derivative."""
+
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2):
+        K = x.shape[-1]
+        # (a frozen fc1 needs nothing of x)
+        q, scale = ops.act8_pack(x.reshape(-1, K)) if ctx.needs_input_grad[1] else (None, None)
+        h, hq, hs = L.tops().act8_gelu_fwd(_forward_gemm(x, w1, b1).reshape(-1, w1.shape[0]), True)
+        ctx.save_for_backward(q, scale, hq, hs, w1, w2)
+        ctx.shape, ctx.has_bias = x.shape, (b1 is not None, b2 is not None)
+        T = h.shape[0]
+        ctx.wt = [_WT.request(w) if _dgrad_on_token_gemm(T, w, x.dtype) else None for w in (w1, w2)]
+        return _forward_gemm(h, w2, b2).view(*x.shape[:-1], w2.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        q, scale, hq, hs, w1, w2 = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gy2 = gy.reshape(-1, gy.shape[-1]).to(w2.dtype)
+        gh, h = L.tops().act8_gelu_bwd(_dgrad_gemm(gy2, w2, ctx.wt[1]), hq, hs, need[3])
+        gw1 = gb1 = gw2 = gb2 = None
+        if need[3]:
+            if ctx.has_bias[1] and need[4]:
+                gw2, gb2 = weight_grad(gy2, h, w2.dtype, bias=True)
+            else:
+                gw2 = weight_grad(gy2, h, w2.dtype)
+        elif ctx.has_bias[1] and need[4]:
+            gb2 = gy2.sum(0, dtype=torch.float32).to(w2.dtype)
+        if need[1]:
+            if ctx.has_bias[0] and need[2]:
+                gw1, gb1 = ops.act8_wgrad(gh, q, scale, w1.shape[1], w1.dtype, bias=True)
+            else:
+                gw1 = ops.act8_wgrad(gh, q, scale, w1.shape[1], w1.dtype)
+        elif ctx.has_bias[0] and need[2]:
+            gb1 = gh.sum(0, dtype=torch.float32).to(w1.dtype)
+        gx = _dgrad_gemm(gh, w1, ctx.wt[0]).view(ctx.shape) if need[0] else None
+        ctx.wt = None
+        return gx, gw1, gb1, gw2, gb2
+
+
+def _act8_ready(x, *params) -> bool:
+    """Whether an act8 Function takes these: a device tensor that a gradient is wanted of, all
+    in one dtype of the kernels'."""
+    return (x.is_cuda and torch.is_grad_enabled() and x.dtype in (torch.float32, torch.bfloat16)
+            and all(p is None or p.dtype == x.dtype for p in params))
+
+
+def linear_act8(x, w, b=None):
+    """F.linear(x, w, b) whose weight gradient reads x's 8-bit checkpoint (ops.act8_pack) instead
+    of x.  Plain F.linear where no weight gradient is wanted: nothing of x is kept then."""
+    if torch.is_autocast_enabled() and x.is_cuda:
+        dt = torch.get_autocast_dtype("cuda")
+        with torch.autocast("cuda", enabled=False):
+            return linear_act8(x.to(dt), w.to(dt), None if b is None else b.to(dt))
+    if not (_act8_ready(x, w, b) and w.requires_grad):
+        return F.linear(x, w, b)
+    return _LinearAct8Fn.apply(x, w, b)
+
+
+def mlp_act8(x, w1, b1, w2, b2):
+    """fc2(gelu(fc1(x))) (exact GELU; w1 [hidden, C], w2 [C', hidden]) that keeps 8-bit
+    checkpoints of x and of the pre-activation and nothing else (see _MlpAct8Fn)."""
+    if torch.is_autocast_enabled() and x.is_cuda:
+        dt = torch.get_autocast_dtype("cuda")
+        with torch.autocast("cuda", enabled=False):
+            return mlp_act8(x.to(dt), *(p if p is None else p.to(dt) for p in (w1, b1, w2, b2)))
+    if not (_act8_ready(x, w1, b1, w2, b2)
+            and any(p is not None and p.requires_grad for p in (x, w1, b1, w2, b2))):
+        return F.linear(F.gelu(F.linear(x, w1, b1)), w2, b2)
+    return _MlpAct8Fn.apply(x, w1, b1, w2, b2)
 
 
 class TokenLinear(nn.Linear):

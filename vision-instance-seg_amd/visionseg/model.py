@@ -29,7 +29,8 @@ import torch.nn.functional as F
 
 from . import ops
 from . import linear as linear_mod
-from .linear import (SmallLinear, TokenLayerNorm, TokenLinear, fp8_operand_ok, in_projection, linear_fp8_tokens,
+from .linear import (SmallLinear, TokenLayerNorm, TokenLinear, fp8_operand_ok, in_projection, linear_act8,
+                     linear_fp8_tokens, mlp_act8,
                      linear_gelu_tokens,
                      linear_relu_tokens, mlp_fp8, linear_tokens, plane_projection, token_plane_projection, self_attn_in_proj, small_linear, value_query_projection,
                      reattach_level_embed)
@@ -68,6 +69,10 @@ class M2FConfig:
     # and K >= linear.FP8_MIN_K) on the block-scaled MX fp8 MFMA (vs_token_gemm; straight-through
     # backward in bf16)
     linear_fp8: bool = False
+    # the Swin blocks keep what their norms, qkv projections and MLPs need for the backward pass
+    # as 8-bit activation checkpoints (ops.act8_pack): same forward results, about half the
+    # activation memory; not together with linear_fp8
+    act8: bool = False
 
     @staticmethod
     def preset(name: str, **kw) -> "M2FConfig":
@@ -130,8 +135,11 @@ class Mlp(nn.Module):
         self.fc1 = TokenLinear(dim, hidden)
         self.fc2 = TokenLinear(hidden, dim)
         self.fp8 = False
+        self.act8 = False
 
     def forward(self, x, xq=None):
+        if self.act8:
+            return mlp_act8(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias)
         if self.fp8:
             return mlp_fp8(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, xq)
         # the GELU output feeds fc2 only: its backward rides in fc2's dX GEMM (ops.GeluBackwardSink)
@@ -146,6 +154,7 @@ class SwinBlock(nn.Module):
         self.ws, self.shift = ws, shift
         self.attn_fp8 = False                  # set by SwinBackbone from M2FConfig.attn_fp8
         self.linear_fp8 = False                # set by SwinBackbone from M2FConfig.linear_fp8
+        self.act8 = False                      # set by SwinBackbone from M2FConfig.act8
         self.norm1 = TokenLayerNorm(dim)
         self.attn = WindowAttention(dim, heads, ws)
         self.norm2 = TokenLayerNorm(dim)
@@ -185,10 +194,12 @@ class SwinBlock(nn.Module):
                 x, h, hq = self.norm1.add_forward_windows(x, res, wr, quant=True)
             qkv = linear_fp8_tokens(h.view(-1, ws * ws, C), self.attn.qkv.weight, self.attn.qkv.bias, hq)
         elif res is None:
-            h = self.norm1.forward_windows(x, wr)
+            h = self.norm1.forward_windows(x, wr, act8=self.act8)
         else:
-            x, h = self.norm1.add_forward_windows(x, res, wr)
-        if not (q8 or r_qkv):
+            x, h = self.norm1.add_forward_windows(x, res, wr, act8=self.act8)
+        if self.act8:
+            qkv = linear_act8(h.view(-1, ws * ws, C), self.attn.qkv.weight, self.attn.qkv.bias)
+        elif not (q8 or r_qkv):
             qkv = (linear_fp8_tokens(h.view(-1, ws * ws, C), self.attn.qkv.weight, self.attn.qkv.bias)
                    if self.linear_fp8 else self.attn.qkv(h.view(-1, ws * ws, C)))
         # output in the image layout (window reverse folded into the kernel); the per-token
@@ -205,7 +216,7 @@ class SwinBlock(nn.Module):
         if q8 or r_fc1:
             x, h2, h2q = self.norm2.add_forward(x, o, quant="rows" if r_fc1 else True)
             return x, self.mlp(h2, h2q)
-        x, h2 = self.norm2.add_forward(x, o)
+        x, h2 = self.norm2.add_forward(x, o, act8=self.act8)
         return x, self.mlp(h2)
 
 
@@ -272,6 +283,8 @@ class SwinBackbone(nn.Module):
 
     def __init__(self, cfg: M2FConfig):
         super().__init__()
+        if cfg.act8 and cfg.linear_fp8:
+            raise ValueError("M2FConfig: act8 and linear_fp8 cannot be combined")
         C = cfg.embed_dim
         n = len(cfg.depths)
         self.patch_embed = PatchEmbed(C)
@@ -283,6 +296,7 @@ class SwinBackbone(nn.Module):
             for blk in st.blocks:
                 blk.attn_fp8 = bool(cfg.attn_fp8)
                 blk.linear_fp8 = blk.mlp.fp8 = bool(cfg.linear_fp8)
+                blk.act8 = blk.mlp.act8 = bool(cfg.act8)
 
     def forward(self, px):
         H, W = px.shape[-2:]
