@@ -316,11 +316,11 @@ VS_API int vs_act8_layer_norm_backward(int dtype, const void* gy, const void* gs
                                        long long gy_count, void* stream);
 
 /* dW[o, i] = sum_t gy[t, o] h[t, i] and, db not NULL, db[o] = sum_t gy[t, o] of a Linear with N
- * outputs and K inputs from its output gradient gy [tokens, N] (dtype; row stride ld_gy, unit
- * feature stride) and the checkpoint of its input (q 16-B aligned): dw [N, K], db [N] in
+ * outputs and K inputs from its output gradient gy [tokens, N] (dtype; row stride ld_gy >= N,
+ * unit feature stride) and the checkpoint of its input (q 16-B aligned): dw [N, K], db [N] in
  * out_dtype (overwritten; 0 where tokens is 0).  f32 accumulation; bf16 gy: exact products;
  * f32 gy: exact products too (three bf16 parts).  K > 0.  Deterministic. */
-VS_API long long vs_act8_wgrad_workspace_bytes(long long tokens, int N, int K);
+VS_API long long vs_act8_wgrad_workspace_bytes(int dtype, long long tokens, int N, int K);
 VS_API int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long ld_gy, const void* q, const void* scale,
                          void* dw, void* db, void* workspace, long long tokens, int N, int K, void* stream);
 

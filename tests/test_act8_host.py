@@ -72,7 +72,7 @@ def test_c_entry_points_refuse():
     refused(lib.vs_act8_wgrad(1, 1, P16, 8, P16, P16, P16, P16, P16, 4, 8, 0, None), b"K > 0")
     refused(lib.vs_act8_wgrad(1, 1, P16, 8, ctypes.c_void_p(24), P16, P16, P16, P16, 4, 8, 8, None), b"aligned")
     refused(lib.vs_act8_wgrad(1, 1, NULL, 8, P16, P16, P16, P16, P16, 4, 8, 8, None), b"null")
-    need = lib.vs_act8_wgrad_workspace_bytes(65536, 64, 64)
+    need = lib.vs_act8_wgrad_workspace_bytes(1, 65536, 64, 64)
     assert need > 0
     refused(lib.vs_act8_wgrad(1, 1, P16, 64, P16, P16, P16, P16, NULL, 65536, 64, 64, None), b"workspace")
     # nothing to do: no pointer is looked at
@@ -81,7 +81,7 @@ def test_c_entry_points_refuse():
     assert lib.vs_act8_gelu_forward(0, NULL, NULL, NULL, NULL, 0, 8, None) == 0
     assert lib.vs_act8_layer_norm_backward_workspace_bytes(0, 64) > 0
     assert lib.vs_act8_layer_norm_backward_workspace_bytes(4, 0) == 0
-    assert lib.vs_act8_wgrad_workspace_bytes(-1, 8, 8) == 0
+    assert lib.vs_act8_wgrad_workspace_bytes(1, -1, 8, 8) == 0
 
 
 def test_ops_refuse_cpu_tensors():

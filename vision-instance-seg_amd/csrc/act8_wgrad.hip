@@ -7,12 +7,13 @@
 // way into LDS, once a workgroup, exactly (act8.h).  f32 gradients are cut into three bf16 parts
 // by truncation, gY = hi + mid + lo: 8 bits of significand each, so the sum is exact, and three
 // matrix products give what an f32 product of exact terms would; a non-finite value is its hi
-// part alone.  Accumulation is f32 in the matrix units.  db comes from one more MFMA an operand
-// tile, with a first operand of ones, in the workgroups of the first input columns.
+// part alone.  Accumulation is f32 in the matrix units.  db is summed on the way into LDS by the
+// workgroups of the first input columns.
 //
-// A workgroup owns 128 output rows x 128 input columns of dW for one split of the tokens.  The
-// next chunk is in flight in registers while one is multiplied; LDS holds two chunks.  Splits
-// write f32 partials that a second kernel adds up in a fixed order (no atomics).
+// A workgroup owns BO output rows x BI input columns of dW for one split of the tokens.  LDS holds
+// two chunks: while chunk c is multiplied, chunk c + 1 goes from registers into LDS and chunk
+// c + 2 from memory into the registers, piece by piece between the MFMAs; one barrier a chunk.
+// Splits write f32 partials that a second kernel adds up in a fixed order (no atomics).
 #include <type_traits>
 
 #include "act8.h"
@@ -21,22 +22,19 @@
 namespace vs {
 namespace {
 
-constexpr int kTK = 64;                          // tokens of a chunk
-constexpr int kThreads = 256;
-constexpr int kImg = kTK * 256;                  // bytes of an image: 64 tokens x 128 bf16
-
 struct Wgrad8 {
   const void* gy;
   const unsigned char* q;
   const unsigned char* scale;
   void* dw;
   void* db;
-  float* part;                                   // [S][tiles][128 * 128] in fragment order (S > 1)
+  float* part;                                   // [S][tiles][BO * BI] in fragment order (S > 1)
   float* pbias;                                  // [S][N]
   long long ldg, T;
   int N, K, P;                                   // P: the checkpoint's pitch
   int S, tiles_i, tiles;
   int f32_out;
+  int vec;                                       // dW's rows take 4-element stores
 };
 
 __device__ __forceinline__ void store_out(void* p, size_t i, bool f32, float v) {
@@ -44,6 +42,23 @@ __device__ __forceinline__ void store_out(void* p, size_t i, bool f32, float v) 
     reinterpret_cast<float*>(p)[i] = v;
   else
     reinterpret_cast<bf16*>(p)[i] = __float2bfloat16(v);
+}
+
+// dW[o, i .. i + 3], as far as it goes
+__device__ __forceinline__ void store_four(const Wgrad8& a, int o, int i, float x, float y, float z, float w) {
+  const size_t at = (size_t)o * a.K + i;
+  if (a.vec && i < a.K) {                        // rows of a multiple of 4: i + 3 < K too
+    if (a.f32_out)
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.dw) + at) = make_float4(x, y, z, w);
+    else
+      *reinterpret_cast<bf16x4_t*>(reinterpret_cast<bf16*>(a.dw) + at) =
+          bf16x4_t{bf16_bits(x), bf16_bits(y), bf16_bits(z), bf16_bits(w)};
+    return;
+  }
+  const float v[4] = {x, y, z, w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < a.K) store_out(a.dw, at + e, a.f32_out, v[e]);
 }
 
 // the bf16 parts of 8 f32 values (truncation; see the head of the file)
@@ -65,184 +80,449 @@ __device__ __forceinline__ void split3(const float* v, uint4& hi, uint4& mid, ui
   lo = make_uint4(two(l, 0), two(l, 2), two(l, 4), two(l, 6));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) act8_wgrad_kernel(const Wgrad8 a) {
+__device__ __forceinline__ uint4 buffer16(__amdgpu_buffer_rsrc_t rs, int offset) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+__device__ __forceinline__ void lds16(lds_byte* p, uint4 a) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 v = {a.x, a.y, a.z, a.w};
+  *(__attribute__((address_space(3))) u32x4*)p = v;
+}
+
+// acc += h^T gY over the wave's TO x TI tiles of 32 x 32, chunk by chunk
+template <typename T, int BO, int BI, int WO, int WI, int TK, bool FAST>
+__global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;   // parts of a gradient
-  constexpr int kStage = (NP + 1) * kImg;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];       // two stages
+  constexpr int NT = 64 * WO * WI, TO = BO / WO / 32, TI = BI / WI / 32;
+  constexpr int kImg = TK * 256;                              // bytes of an image: TK tokens x 128 bf16
+  constexpr int NHO = BO / 128, NHI = BI / 128;               // images of a part of gY, of h
+  constexpr int kStage = (NP * NHO + NHI) * kImg;
+  constexpr int GC = BO / 8, XC = BI / 16;                    // pieces of a token: 8 gradients, 16 of q
+  constexpr int GP = TK * GC / NT, XP = TK * XC / NT;         // pieces of a thread
+  constexpr int KS = TK / 16;                                 // MFMA steps of a chunk
+  static_assert(GP * NT == TK * GC && XP * NT == TK * XC && NT % GC == 0 && NT % (2 * XC) == 0, "whole pieces");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int wg = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int s = wg / a.tiles, tile = wg - s * a.tiles;
+  const int s = wg / a.tiles, tile = wg - s * a.tiles;        // a split's tiles are neighbours (one XCD's L2)
   const int ob = tile / a.tiles_i, ib = tile - ob * a.tiles_i;
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63, r = l & 31, hh = l >> 5;
-  const int wo = (w & 1) * 64, wi = (w >> 1) * 64;            // this wave's 64 x 64
-  const long long nchunk = (a.T + kTK - 1) / kTK;
-  const long long cb = nchunk * s / a.S, ce = nchunk * (s + 1) / a.S;
-  const bool do_bias = a.db != nullptr && ib == 0 && (w >> 1) == 0;
-  const T* gy = reinterpret_cast<const T*>(a.gy);
+  const int qo = w % WO, qi = w / WO;
+  const int wo = qo * (BO / WO), wi = qi * (BI / WI);
+  const int nchunk = (int)((a.T + TK - 1) / TK);
+  const int cb = (int)((long long)nchunk * s / a.S), ce = (int)((long long)nchunk * (s + 1) / a.S);
+  const bool do_bias = a.db != nullptr && ib == 0;
 
-  // a chunk's pieces of this thread: 4 x 8 gradients (row = piece * 16 + tid / 16, columns 8 (tid
-  // & 15)..), 2 x 16 bytes of the checkpoint (row = piece * 32 + tid / 8, columns 16 (tid & 7)..)
-  const int gc = 8 * (threadIdx.x & 15), gr = threadIdx.x >> 4;
-  const int xc = 16 * (threadIdx.x & 7), xr = threadIdx.x >> 3;
-  const int gcol = ob * 128 + gc, xcol = ib * 128 + xc;
-  const bool xin = xcol < a.P;
-  Chunk<T> g[4];
-  uint4 xq[2];
-  uint32_t xs[2];
-  auto fetch = [&](long long c) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const long long t = c * kTK + p * 16 + gr;
-      if (t < a.T)
-        load_row_chunk(g[p], gy + t * a.ldg, gcol >> 3, a.N);
+  const int gr = threadIdx.x / GC, gc = threadIdx.x % GC, xr = threadIdx.x / XC, xc = threadIdx.x % XC;
+  const int gcol = ob * BO + gc * 8, xcol = ib * BI + xc * 16;
+  Chunk<T> g[GP];
+  uint4 xq[XP];
+  uint32_t xs[XP];
+  // The next chunk to fetch: the three tensors from its first row on, and the rows left.  A buffer
+  // load gives 0 behind the chunk's last row, which are the tokens behind the last one; columns
+  // behind N or P hold whatever is there (the next row): they only reach rows and columns of dW
+  // that do not exist.
+  const long long cb_rows = (long long)cb * TK;
+  const unsigned char* gbase = reinterpret_cast<const unsigned char*>(a.gy) + cb_rows * a.ldg * (long long)sizeof(T);
+  const unsigned char* qbase = a.q + cb_rows * a.P;
+  const unsigned char* sbase = a.scale + cb_rows * (a.P >> 5);
+  const long long end = (long long)ce * TK;      // (behind the split's last chunk too: zeros)
+  int left = (int)((end < a.T ? end : a.T) - cb_rows);
+  const int gld = (int)(a.ldg * (long long)sizeof(T)), sld = a.P >> 5;        // (gld: the FAST path's)
+  const int goff = gr * gld + gcol * (int)sizeof(T), xoff = xr * a.P + xcol, soff = xr * sld + (xcol >> 5);
+  const int gap = gld - ((a.N * (int)sizeof(T) + 3) & ~3);                    // behind a row's last dword
+  // the chunk's bytes (readfirstlane: buffer descriptors live in scalar registers)
+  int gsize, qsize, ssize;
+  auto size_up = [&]() {
+    const int rows = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : left < TK ? left : TK);
+    const int g0 = rows * gld - gap;
+    gsize = __builtin_amdgcn_readfirstlane(g0 < 0 ? 0 : g0);
+    qsize = rows * a.P;
+    ssize = rows * sld;
+  };
+  size_up();
+  auto fetch_g = [&](int p) {
+    if constexpr (FAST) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)gbase, 0, gsize, 0x00020000);
+      g[p].a = buffer16(rs, goff + p * (NT / GC) * gld);
+      if constexpr (NP == 3) g[p].b = buffer16(rs, goff + p * (NT / GC) * gld + 16);
+    } else {
+      const int row = p * (NT / GC) + gr;
+      if (row < left)
+        load_row_chunk(g[p], reinterpret_cast<const T*>(gbase) + row * a.ldg, gcol >> 3, a.N);
       else
         g[p].zero();
     }
+  };
+  auto fetch_x = [&](int p) {
+    const auto rq = __builtin_amdgcn_make_buffer_rsrc((void*)qbase, 0, qsize, 0x00020000);
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)sbase, 0, ssize, 0x00020000);
+    xq[p] = buffer16(rq, xoff + p * (NT / XC) * a.P);
+    xs[p] = __builtin_amdgcn_raw_buffer_load_b8(rs, soff + p * (NT / XC) * sld, 0, 0);
+  };
+  auto advance = [&]() {
+    gbase += TK * a.ldg * (long long)sizeof(T);
+    qbase += (long long)TK * a.P;
+    sbase += (long long)TK * sld;
+    left -= TK;
+    size_up();
+  };
+  // LDS addresses, all of the current stage: the pieces' places (a piece's rows are 16 apart or a
+  // multiple: the swizzle is the same) and the operands' (tr_frag: rows k.., 4 rows on, columns)
+  typedef __attribute__((address_space(3))) bf16x4v_t lds_v4;
+  constexpr int GD = (NT / GC) % 16 == 0 ? 1 : 2;
+  static_assert((NT / GC) * GD % 16 == 0 && (NT / XC) % 16 == 0, "a thread's pieces have one swizzle");
+  lds_byte* const base = (lds_byte*)smem;
+  lds_byte* at_g[GD];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const long long t = c * kTK + p * 32 + xr;
-      xq[p] = make_uint4(0u, 0u, 0u, 0u);
-      xs[p] = 1u;
-      if (t < a.T && xin) {
-        xq[p] = *reinterpret_cast<const uint4*>(a.q + t * a.P + xcol);
-        xs[p] = a.scale[t * (a.P >> 5) + (xcol >> 5)];
+  for (int d = 0; d < GD; ++d) at_g[d] = base + (gc >> 4) * kImg + woff(gr + d * (NT / GC), gc & 15);
+  // four neighbouring lanes write the first 16-B half of their pieces of q first, the next four the
+  // second: eight lanes then cover 128 B of banks
+  const bool swap = (xc >> 2) & 1;
+  lds_byte* at_x[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    at_x[h] = base + (NP * NHO + (xc >> 3)) * kImg + woff(xr, 2 * (xc & 7) + ((h == 1) != swap ? 1 : 0));
+  lds_byte *at_b[TO][2], *at_a[TI][2];
+  {
+    const int row = 8 * hh + ((l & 15) >> 2), col = (l & 16) + 4 * (l & 3);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int to = 0; to < TO; ++to) {
+        const int c = ((wo + 32 * to) & 127) + col;
+        at_b[to][h] = base + ((wo + 32 * to) >> 7) * kImg + woff(row + 4 * h, c >> 3) + (c & 7) * 2;
       }
+#pragma unroll
+      for (int ti = 0; ti < TI; ++ti) {
+        const int c = ((wi + 32 * ti) & 127) + col;
+        at_a[ti][h] = base + (NP * NHO + ((wi + 32 * ti) >> 7)) * kImg + woff(row + 4 * h, c >> 3) + (c & 7) * 2;
+      }
+    }
+  }
+  float bsum[8];                                 // this thread's columns of gY, summed as they pass
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bsum[i] = 0.f;
+  auto put_g = [&](int p, auto bias_tag) {
+    constexpr bool BIAS = decltype(bias_tag)::value;
+    lds_byte* to = at_g[p % GD] + (p / GD) * GD * (NT / GC) * 256;
+    if constexpr (NP == 3 || BIAS) {
+      float v[8];
+      g[p].unpack(v);
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bsum[i] += v[i];
+      }
+      if constexpr (NP == 3) {
+        uint4 hi, mid, lo;
+        split3(v, hi, mid, lo);
+        lds16(to, hi);
+        lds16(to + NHO * kImg, mid);
+        lds16(to + 2 * NHO * kImg, lo);
+      }
+    }
+    if constexpr (NP == 1) lds16(to, g[p].a);
+  };
+  auto put_x = [&](int p) {
+    const uint2 lo = make_uint2(xq[p].x, xq[p].y), hi = make_uint2(xq[p].z, xq[p].w);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+      const bool second = (h == 1) != swap;
+      unpack_chunk(make_uint2(second ? hi.x : lo.x, second ? hi.y : lo.y), xs[p], v);
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)                // exact in bf16: the upper halves
+        o[i] = __builtin_amdgcn_perm(__float_as_uint(v[2 * i + 1]), __float_as_uint(v[2 * i]), 0x07060302u);
+      lds16(at_x[h] + p * (NT / XC) * 256, make_uint4(o[0], o[1], o[2], o[3]));
     }
   };
-  auto put = [&](int st) {
-    unsigned char* base = smem + st * kStage;
+  auto to_stage = [&](int step) {                // where the pieces go, `step` stages on
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int at = woff(p * 16 + gr, gc >> 3);
-      if constexpr (NP == 1) {
-        *reinterpret_cast<uint4*>(base + at) = g[p].a;
-      } else {
-        float v[8];
-        uint4 hi, mid, lo;
-        g[p].unpack(v);
-        split3(v, hi, mid, lo);
-        *reinterpret_cast<uint4*>(base + at) = hi;
-        *reinterpret_cast<uint4*>(base + kImg + at) = mid;
-        *reinterpret_cast<uint4*>(base + 2 * kImg + at) = lo;
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint2 half[2] = {make_uint2(xq[p].x, xq[p].y), make_uint2(xq[p].z, xq[p].w)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-        unpack_chunk(half[h], xs[p], v);
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)              // exact in bf16: the upper halves
-          o[i] = __builtin_amdgcn_perm(__float_as_uint(v[2 * i + 1]), __float_as_uint(v[2 * i]), 0x07060302u);
-        *reinterpret_cast<uint4*>(base + NP * kImg + woff(p * 32 + xr, (xc >> 3) + h)) =
-            make_uint4(o[0], o[1], o[2], o[3]);
-      }
-    }
+    for (int d = 0; d < GD; ++d) at_g[d] += step * kStage;
+    at_x[0] += step * kStage;
+    at_x[1] += step * kStage;
   };
 
-  f32x16_t acc[2][2], accb[2];
+  f32x16_t acc[TO][TI];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    zero16(accb[x]);
-    zero16(acc[x][0]);
-    zero16(acc[x][1]);
-  }
-  const short one = (short)0x3f80;               // bf16 1.0
-  const bf16x8_t ones = {one, one, one, one, one, one, one, one};
-  if (cb < ce) fetch(cb);
-  for (long long c = cb; c < ce; ++c) {
-    const int st = (int)(c - cb) & 1;
-    put(st);
-    __syncthreads();                             // stage st is whole; stage st ^ 1 was read before it
-    if (c + 1 < ce) fetch(c + 1);
-    const unsigned char* sg = smem + st * kStage;
-    const unsigned char* sx = sg + NP * kImg;
+  for (int x = 0; x < TO; ++x)
 #pragma unroll
-    for (int k = 0; k < kTK / 16; ++k) {
-      bf16x8_t xa[2];
+    for (int y = 0; y < TI; ++y) zero16(acc[x][y]);
+
+  auto run = [&](auto bias_tag) {
+    // the first chunk into LDS, the next one into the registers
 #pragma unroll
-      for (int ti = 0; ti < 2; ++ti) xa[ti] = tr_frag(sx, 16 * k, wi + 32 * ti, l);
+    for (int j = 0; j < 2; ++j) {
+      if (j == 1) {
 #pragma unroll
-      for (int to = 0; to < 2; ++to)
+        for (int p = 0; p < GP; ++p) put_g(p, bias_tag);
 #pragma unroll
-        for (int p = NP - 1; p >= 0; --p) {      // the smallest part first
-          const bf16x8_t gb = tr_frag(sg + p * kImg, 16 * k, wo + 32 * to, l);
+        for (int p = 0; p < XP; ++p) put_x(p);
+        to_stage(1);
+      }
 #pragma unroll
-          for (int ti = 0; ti < 2; ++ti) acc[to][ti] = mfma16(xa[ti], gb, acc[to][ti]);
-          if (do_bias) accb[to] = mfma16(ones, gb, accb[to]);
+      for (int p = 0; p < GP; ++p) fetch_g(p);
+#pragma unroll
+      for (int p = 0; p < XP; ++p) fetch_x(p);
+      advance();
+    }
+    lds_barrier();
+    // operands of a step of 16 tokens, read one step ahead
+    bf16x8_t xa[2][TI], gb[2][TO][NP];
+    auto operand = [&](lds_byte* const (&p)[2], int offset) {
+      const bf16x4v_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p[0] + offset));
+      const bf16x4v_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p[1] + offset));
+      return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto read = [&](int k, int f) {
+#pragma unroll
+      for (int ti = 0; ti < TI; ++ti) xa[f][ti] = operand(at_a[ti], 16 * 256 * k);
+#pragma unroll
+      for (int to = 0; to < TO; ++to)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) gb[f][to][p] = operand(at_b[to], p * NHO * kImg + 16 * 256 * k);
+    };
+    auto next_stage = [&](int step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int to = 0; to < TO; ++to) at_b[to][h] += step * kStage;
+#pragma unroll
+        for (int ti = 0; ti < TI; ++ti) at_a[ti][h] += step * kStage;
+      }
+    };
+    static_assert(KS % 2 == 0, "the operands' two sets alternate over chunks");
+    int flip = 1;                                // from the stage that is read to the other one
+    read(0, 0);
+    for (int c = cb; c < ce; ++c) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (k + 1 < KS) {
+          read(k + 1, (k + 1) & 1);
+        } else {
+          // chunk c's last operands are in registers and chunk c + 1 is written: the barrier makes
+          // it visible and its own place free, with the last step's MFMAs still to issue
+          if constexpr (TO * TI >= 8) {
+            // the steps before, MFMA by MFMA with a share of the operand reads and of the pieces'
+            // arithmetic behind each (1257 ns a chunk against 1374 as the compiler has it, and 44
+            // against 45 us at 16384 x 1536 x 384; the smaller tiles lose by it)
+#pragma unroll
+            for (int i = 0; i < (KS - 1) * TO * TI; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);      // MFMA
+              __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);      // vector arithmetic
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);    // LDS reads
+            }
+          }
+          lds_barrier();                         // (the loads of chunk c + 2 stay in flight)
+          next_stage(flip);
+          read(0, 0);
         }
+        const int f = k & 1;
+#pragma unroll
+        for (int to = 0; to < TO; ++to)
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p)      // the smallest part first
+#pragma unroll
+            for (int ti = 0; ti < TI; ++ti) acc[to][ti] = mfma16(xa[f][ti], gb[f][to][p], acc[to][ti]);
+        // (behind the last chunk too: into places that are not read again)
+        constexpr int PS = KS - 1;               // the steps that carry the pieces
+        if (k < PS) {
+#pragma unroll
+          for (int p = GP * k / PS; p < GP * (k + 1) / PS; ++p) put_g(p, bias_tag);
+#pragma unroll
+          for (int p = XP * k / PS; p < XP * (k + 1) / PS; ++p) put_x(p);
+#pragma unroll
+          for (int p = GP * k / PS; p < GP * (k + 1) / PS; ++p) fetch_g(p);
+#pragma unroll
+          for (int p = XP * k / PS; p < XP * (k + 1) / PS; ++p) fetch_x(p);
+        }
+      }
+      advance();
+      to_stage(-flip);
+      flip = -flip;
+    }
+    lds_barrier();
+  };
+  if (do_bias)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
+  if (do_bias) {                                 // the threads that hold the same columns, in order
+    float* sum = reinterpret_cast<float*>(smem);
+    constexpr int R = NT / GC;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[gr * BO + gc * 8 + i] = bsum[i];
+    __syncthreads();
+    const int o = ob * BO + (int)threadIdx.x;
+    if ((int)threadIdx.x < BO && o < a.N) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < R; ++k) t += sum[k * BO + threadIdx.x];
+      if (a.S > 1)
+        a.pbias[(size_t)s * a.N + o] = t;
+      else
+        store_out(a.db, o, a.f32_out, t);
     }
   }
 
   // C tile: lane column = o, registers 4 g.. = 4 consecutive i
   if (a.S > 1) {
-    float* pw = a.part + ((size_t)s * a.tiles + tile) * (128 * 128) + (size_t)w * 4096 + l * 4;
+    float* pw = a.part + ((size_t)s * a.tiles + tile) * (BO * BI) + (size_t)w * (TO * TI * 1024) + l * 4;
 #pragma unroll
-    for (int to = 0; to < 2; ++to)
+    for (int to = 0; to < TO; ++to)
 #pragma unroll
-      for (int ti = 0; ti < 2; ++ti)
+      for (int ti = 0; ti < TI; ++ti)
 #pragma unroll
         for (int gq = 0; gq < 4; ++gq)
-          *reinterpret_cast<float4*>(pw + ((to * 2 + ti) * 4 + gq) * 256) = make_float4(
+          *reinterpret_cast<float4*>(pw + ((to * TI + ti) * 4 + gq) * 256) = make_float4(
               acc[to][ti][4 * gq], acc[to][ti][4 * gq + 1], acc[to][ti][4 * gq + 2], acc[to][ti][4 * gq + 3]);
   }
 #pragma unroll
-  for (int to = 0; to < 2; ++to) {
-    const int o = ob * 128 + wo + 32 * to + r;
+  for (int to = 0; to < TO; ++to) {
+    const int o = ob * BO + wo + 32 * to + r;
     if (o >= a.N) continue;
     if (a.S == 1) {
 #pragma unroll
-      for (int ti = 0; ti < 2; ++ti)
+      for (int ti = 0; ti < TI; ++ti)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = ib * 128 + wi + 32 * ti + crow(e, hh);
-          if (i < a.K) store_out(a.dw, (size_t)o * a.K + i, a.f32_out, acc[to][ti][e]);
-        }
-    }
-    if (do_bias && hh == 0) {
-      if (a.S > 1)
-        a.pbias[(size_t)s * a.N + o] = accb[to][0];
-      else
-        store_out(a.db, o, a.f32_out, accb[to][0]);
+        for (int gq = 0; gq < 4; ++gq)
+          store_four(a, o, ib * BI + wi + 32 * ti + 8 * gq + 4 * hh, acc[to][ti][4 * gq], acc[to][ti][4 * gq + 1],
+                     acc[to][ti][4 * gq + 2], acc[to][ti][4 * gq + 3]);
     }
   }
 }
 
-// dW[o][i] = the splits' partials added in order; db likewise
-__global__ void __launch_bounds__(kThreads) act8_wgrad_sum_kernel(const Wgrad8 a) {
-  const long long at = (long long)blockIdx.x * kThreads + threadIdx.x, n = (long long)a.N * a.K;
-  if (at < n) {
-    const int o = (int)(at / a.K), i = (int)(at - (long long)o * a.K);
-    const int oo = o & 127, ii = i & 127, row = ii & 31;
-    const int wv = (oo >> 6) | ((ii >> 6) << 1), to = (oo >> 5) & 1, ti = (ii >> 5) & 1;
-    const int lane = (oo & 31) + 32 * ((row >> 2) & 1), e = (row & 3) + 4 * (row >> 3);
-    const float* p = a.part + ((size_t)(o >> 7) * a.tiles_i + (i >> 7)) * (128 * 128) + (size_t)wv * 4096 +
-                     ((to * 2 + ti) * 4 + (e >> 2)) * 256 + lane * 4 + (e & 3);
-    float v = 0.f;
-    for (int s = 0; s < a.S; ++s) v += p[(size_t)s * a.tiles * (128 * 128)];
-    store_out(a.dw, at, a.f32_out, v);
-  } else if (a.db && at - n < a.N) {
-    float v = 0.f;
-    for (int s = 0; s < a.S; ++s) v += a.pbias[(size_t)s * a.N + (at - n)];
-    store_out(a.db, at - n, a.f32_out, v);
+// dW = the splits' partials added in order, in the partials' own order: a wave reads 1 KB (the
+// 32 x 8 values of a register group) of each split at a time.  A workgroup takes 64 float4 in
+// NG interleaved slices of the splits, whose sums it adds in order; the workgroups behind dW's
+// do the same for db.
+template <int BO, int BI, int WO, int WI, int NG>
+__global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a) {
+  constexpr int TO = BO / WO / 32, TI = BI / WI / 32, GROUPS = BO * BI / 256;
+  __shared__ float4 lds[NG][64];
+  const int l = threadIdx.x & 63, sl = threadIdx.x >> 6;
+  const long long n = (long long)a.tiles * GROUPS;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (blockIdx.x >= n) {
+    const long long o = (blockIdx.x - n) * 64 + l;
+    if (o < a.N)
+      for (int s = sl; s < a.S; s += NG) v.x += a.pbias[(size_t)s * a.N + o];
+    lds[sl][l] = v;
+    __syncthreads();
+    if (sl == 0 && o < a.N) {
+      float t = v.x;
+#pragma unroll
+      for (int k = 1; k < NG; ++k) t += lds[k][l].x;
+      store_out(a.db, o, a.f32_out, t);
+    }
+    return;
+  }
+  const int tile = blockIdx.x / GROUPS, grp = blockIdx.x - tile * GROUPS;
+  const int ob = tile / a.tiles_i, ib = tile - ob * a.tiles_i;
+  const int gq = grp & 3, t = (grp >> 2) % (TO * TI), w = (grp >> 2) / (TO * TI);
+  const int o = ob * BO + (w % WO) * (BO / WO) + 32 * (t / TI) + (l & 31);
+  const int i = ib * BI + (w / WO) * (BI / WI) + 32 * (t % TI) + 8 * gq + 4 * (l >> 5);
+  const float* p = a.part + (size_t)blockIdx.x * 256 + l * 4;
+  const size_t stride = (size_t)a.tiles * BO * BI;
+  if (o < a.N && i < a.K) {
+#pragma unroll 4
+    for (int s = sl; s < a.S; s += NG) {
+      const float4 u = *reinterpret_cast<const float4*>(p + s * stride);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+    }
+  }
+  lds[sl][l] = v;
+  __syncthreads();
+  if (sl == 0 && o < a.N) {
+#pragma unroll
+    for (int k = 1; k < NG; ++k) {
+      const float4 u = lds[k][l];
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+    }
+    store_four(a, o, i, v.x, v.y, v.z, v.w);
   }
 }
 
-// splits of the tokens: enough workgroups for the chip, at least 4 chunks each
-int splits_of(long long T, int N, int K) {
-  const long long tiles = (long long)((N + 127) / 128) * ((K + 127) / 128);
-  const long long nchunk = (T + kTK - 1) / kTK;
-  long long s = (512 + tiles - 1) / tiles;
-  if (s > nchunk / 4) s = nchunk / 4;
-  return (int)(s < 1 ? 1 : s);
+// How a problem is run: the tile and the splits of the tokens, whichever has the smallest estimate
+//     chunks of a workgroup x time of a chunk on a full chip + 4 us
+//     + with splits: 5 us for the second launch and 0.2 us a MB of partials
+// (us; a place is a workgroup that runs at a time: splits fill the places once, or a half, a
+// quarter, ... of them).  Measured as tile 0 / 1 / 2, us:  147456 tokens x 1024 x 2048: 635 / 677 /
+// 790;  65536 x 768 x 192: 48 / 42 / 52;  16384 x 1536 x 384: 45 / 37 / 41;  262144 x 96 x 384: 79 /
+// 67 / 52;  400 x 256 x 256: 20 / 13 / 9.5 (12 in two splits).  f32, tile 3 / 4: 65536 x 768 x 768:
+// 284 / 264;  10007 x 304 x 203: 21 / 23.
+struct Tile {
+  int f32, bo, bi, tk, places;
+  float chunk;
+};
+constexpr Tile kTiles[] = {
+    {0, 256, 256, 64, 256, 2.19f}, {0, 256, 128, 64, 256, 1.175f}, {0, 128, 128, 64, 256, 0.8f},
+    {1, 128, 128, 64, 256, 1.85f}, {1, 128, 128, 32, 512, 1.75f},
+};
+struct Plan {
+  int tile, bo, bi, S;
+  long long tiles;
+};
+
+Plan plan_of(bool f32, long long T, int N, int K) {
+  Plan best = {};
+  float least = 0.f;
+  for (int c = 0; c < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++c) {
+    const Tile& t = kTiles[c];
+    if ((t.f32 != 0) != f32) continue;
+    const long long tiles = (long long)((N + t.bo - 1) / t.bo) * ((K + t.bi - 1) / t.bi);
+    const long long nchunk = (T + t.tk - 1) / t.tk;
+    long long S = t.places / tiles;
+    if (S > nchunk / 2) S = nchunk / 2;
+    if (S < 1) S = 1;
+    for (; S >= 1; S >>= 1) {
+      const long long turns = (tiles * S + t.places - 1) / t.places;
+      float cost = (float)(turns * ((nchunk + S - 1) / S)) * t.chunk + 4.f;
+      if (S > 1) cost += 5.f + 0.2e-6f * (float)(4 * S * tiles * t.bo * t.bi);
+      if (best.S == 0 || cost < least) {
+        best = {c, t.bo, t.bi, (int)S, tiles};
+        least = cost;
+      }
+    }
+  }
+  return best;
 }
 
 bool sizes_ok(long long T, int N, int K) {
-  return T >= 0 && T < (1ll << 40) && N >= 0 && K >= 0 && N <= (1 << 24) && K <= (1 << 24) &&
-         (long long)((N + 127) / 128) * ((K + 127) / 128) < (1 << 22);
+  return T >= 0 && T < (1ll << 31) && N >= 0 && K >= 0 && N <= (1 << 24) && K <= (1 << 24) &&
+         (long long)((N + 127) / 128) * ((K + 127) / 128) < (1 << 20);
+}
+
+long long workspace_bytes(const Plan& p, int N) {
+  return p.S == 1 ? 0 : 4ll * p.S * (p.tiles * p.bo * p.bi + N);
+}
+
+template <typename T, int BO, int BI, int WO, int WI, int TK>
+int launch(const Wgrad8& a, bool fast, hipStream_t st) {
+  constexpr int NP = std::is_same<T, float>::value ? 3 : 1;
+  constexpr int kLds = 2 * (NP * BO / 128 + BI / 128) * TK * 256;
+  const auto kernel = fast ? act8_wgrad_kernel<T, BO, BI, WO, WI, TK, true>
+                           : act8_wgrad_kernel<T, BO, BI, WO, WI, TK, false>;
+  if (kLds > 64 * 1024)                          // above the default limit of a launch
+    VS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.S * a.tiles)), dim3(64 * WO * WI), kLds, st, a);
+  VS_LAUNCH_CHECK();
+  if (a.S > 1) {
+    constexpr int NG = 4;
+    const long long groups = (long long)a.tiles * (BO * BI / 256) + (a.db ? (a.N + 63) / 64 : 0);
+    hipLaunchKernelGGL((act8_wgrad_sum_kernel<BO, BI, WO, WI, NG>), dim3((unsigned)groups), dim3(64 * NG), 0, st, a);
+    VS_LAUNCH_CHECK();
+  }
+  return VS_OK;
 }
 
 }  // namespace
@@ -250,12 +530,9 @@ bool sizes_ok(long long T, int N, int K) {
 
 using namespace vs;
 
-extern "C" long long vs_act8_wgrad_workspace_bytes(long long tokens, int N, int K) {
+extern "C" long long vs_act8_wgrad_workspace_bytes(int dtype, long long tokens, int N, int K) {
   if (!sizes_ok(tokens, N, K) || N == 0 || K == 0) return 0;
-  const long long S = splits_of(tokens, N, K);
-  if (S == 1) return 0;
-  const long long tiles = (long long)((N + 127) / 128) * ((K + 127) / 128);
-  return 4 * S * (tiles * 128 * 128 + N);
+  return workspace_bytes(plan_of(dtype == VS_F32, tokens, N, K), N);
 }
 
 extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long ld_gy, const void* q,
@@ -265,7 +542,8 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
            "dtypes must be VS_F32 or VS_BF16");
   VS_CHECK(sizes_ok(tokens, N, K), "sizes out of range");
   if (N == 0) return VS_OK;
-  VS_CHECK(ld_gy >= 0, "row stride >= 0");
+  if (tokens <= 1) ld_gy = (N + 7) & ~7;         // one row: its stride is not used
+  VS_CHECK(ld_gy >= N, "row stride >= N");
   VS_CHECK((K == 0 || dw) && (tokens == 0 || (gy && (K == 0 || (q && scale)))), "null pointer");
   VS_CHECK(((uintptr_t)q & 15) == 0, "q must be 16-B aligned");
   VS_CHECK(K > 0, "K > 0");
@@ -280,30 +558,25 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
   a.N = N;
   a.K = K;
   a.P = padded32(K);
-  a.S = splits_of(tokens, N, K);
-  a.tiles_i = (K + 127) / 128;
-  a.tiles = ((N + 127) / 128) * a.tiles_i;
+  const Plan plan = plan_of(dtype == VS_F32, tokens, N, K);
+  a.S = plan.S;
+  a.tiles_i = (K + plan.bi - 1) / plan.bi;
+  a.tiles = (int)plan.tiles;
   a.f32_out = out_dtype == VS_F32;
+  a.vec = K % 4 == 0 && ((uintptr_t)dw & 15) == 0;
   VS_CHECK(a.S == 1 || (workspace && ((uintptr_t)workspace & 15) == 0),
            "workspace: 16-B aligned, sized by vs_act8_wgrad_workspace_bytes");
   a.part = (float*)workspace;
-  a.pbias = a.part + (size_t)a.S * a.tiles * (128 * 128);
+  a.pbias = a.part + (size_t)a.S * a.tiles * (plan.bo * plan.bi);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(a.S * a.tiles));
-  if (dtype == VS_BF16) {
-    hipLaunchKernelGGL((act8_wgrad_kernel<bf16>), grid, dim3(kThreads), 4 * kImg, st, a);
-  } else {
-    // 128 KB of LDS: above the default limit of a launch
-    VS_HIP(hipFuncSetAttribute((const void*)act8_wgrad_kernel<float>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               8 * kImg));
-    hipLaunchKernelGGL((act8_wgrad_kernel<float>), grid, dim3(kThreads), 8 * kImg, st, a);
+  // buffer loads: aligned rows, and a chunk of rows within their 32-bit offsets
+  const long long esz = dtype == VS_F32 ? 4 : 2;
+  const bool fast = ((uintptr_t)gy & 15) == 0 && ld_gy * esz % 16 == 0 && 64 * (ld_gy + N) * esz < (1ll << 31);
+  switch (plan.tile) {
+    case 0: return launch<bf16, 256, 256, 2, 4, 64>(a, fast, st);
+    case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, fast, st);
+    case 2: return launch<bf16, 128, 128, 2, 4, 64>(a, fast, st);
+    case 3: return launch<float, 128, 128, 2, 4, 64>(a, fast, st);
+    default: return launch<float, 128, 128, 2, 2, 32>(a, fast, st);
   }
-  VS_LAUNCH_CHECK();
-  if (a.S > 1) {
-    const long long items = (long long)N * K + (db ? N : 0);
-    hipLaunchKernelGGL(act8_wgrad_sum_kernel, dim3((unsigned)((items + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                       st, a);
-    VS_LAUNCH_CHECK();
-  }
-  return VS_OK;
 }

@@ -133,7 +133,7 @@ SIGNATURES = {
                                                           ctypes.c_longlong, _P],
     "vs_act8_layer_norm_backward_workspace_bytes": [ctypes.c_longlong, _c_int],
     "vs_act8_layer_norm_backward": [_c_int] + [_P] * 11 + [ctypes.c_longlong, _c_int, _P, ctypes.c_longlong, _P],
-    "vs_act8_wgrad_workspace_bytes": [ctypes.c_longlong, _c_int, _c_int],
+    "vs_act8_wgrad_workspace_bytes": [_c_int, ctypes.c_longlong, _c_int, _c_int],
     "vs_act8_wgrad": [_c_int, _c_int, _P, ctypes.c_longlong] + [_P] * 5 + [ctypes.c_longlong, _c_int, _c_int, _P],
     "vs_conv3x3_forward": [_P, _P, _P, _P] + [_c_int] * 5 + [_P],
     "vs_conv3x3_weight_layouts": [_P, _P, _P, _c_int, _c_int, _P],
