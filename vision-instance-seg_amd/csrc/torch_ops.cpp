@@ -7,13 +7,16 @@
 // inside an op (msda_*: spatial_shapes / level_start_index are read on the host; pass CPU
 // int64 tensors -- a device tensor costs one device->host copy, as the upstream extension's
 // callers do with `.tolist()`), no global state.  The autograd wrappers stay in Python
-// (visionseg/ops.py), as the upstream `MSDeformAttnFunction` wraps its extension.
+// (visionseg/ops.py), as the upstream `MSDeformAttnFunction` wraps its extension, but for those of
+// the 8-bit activation checkpoints (below: host time).
 // There is no CPU kernel: a CPU tensor is refused (no fallback path exists).
 //
 // Host-only C++ (g++), linked against libvisionseg_hip.so; the kernels live in csrc/*.hip.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -665,6 +668,123 @@ std::tuple<at::Tensor, at::Tensor> act8_wgrad(const at::Tensor& grad_y, const at
   return {dw, db};
 }
 
+// ---- their autograd forms.  C++ Functions, not Python ones as for the ops above: a call on a few
+// hundred rows is all host time, and a Python forward and backward (144 us for a LayerNorm step on
+// 400 rows of 256) cost several times what these do.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that are not differentiable again: under create_graph a second backward through them
+// raises (as torch.autograd.function.once_differentiable has it).
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const auto& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "an op of 8-bit activation checkpoints is differentiated twice: its gradients are once differentiable",
+      in.size());
+  return (*error)(std::move(in));
+}
+
+bool keeps(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+struct GeluAct8 : public torch::autograd::Function<GeluAct8> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x) {
+    auto [y, q, scale] = act8_gelu_fwd(x, true);
+    ctx->save_for_backward({q, scale});
+    ctx->saved_data["dtype"] = x.scalar_type();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor gx;
+    {
+      at::NoGradGuard guard;
+      gx = std::get<0>(act8_gelu_bwd(grads[0].to(ctx->saved_data["dtype"].toScalarType()), saved[0], saved[1], false));
+    }
+    return once({gx});
+  }
+};
+
+at::Tensor gelu_act8(const at::Tensor& x) {
+  return keeps({&x}) ? GeluAct8::apply(x) : std::get<0>(act8_gelu_fwd(x, false));
+}
+
+// the rows of y that no row of x goes to (the window layout's padding) are zeros
+void clear_rows(at::Tensor& y, const std::optional<at::Tensor>& pad) {
+  if (pad.has_value() && pad->numel()) y.index_fill_(0, *pad, 0);
+}
+
+std::optional<at::Tensor> maybe(const at::Tensor& t) {
+  return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+}
+
+// -> y, or with r: s and y
+struct LayerNormAct8 : public torch::autograd::Function<LayerNormAct8> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& r,
+                               const at::Tensor& weight, const at::Tensor& bias, double eps,
+                               const std::optional<at::Tensor>& rows, const std::optional<at::Tensor>& pad,
+                               int64_t out_rows) {
+    ctx->set_materialize_grads(false);
+    auto [s, y, q, scale, mean, rstd] = act8_layer_norm_fwd(x, r, weight, bias, eps, rows, out_rows, true);
+    clear_rows(y, pad);
+    ctx->save_for_backward({q, scale, weight, mean, rstd, rows.value_or(at::Tensor())});
+    ctx->saved_data["residual"] = r.has_value();
+    return r.has_value() ? variable_list{s, y} : variable_list{y};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const at::Tensor gs = residual ? grads[0] : at::Tensor(), gy = residual ? grads[1] : grads[0];
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &scale = saved[1], &weight = saved[2], &mean = saved[3], &rstd = saved[4],
+                     &rows = saved[5];
+    at::Tensor gx, gw, gb;
+    {
+      at::NoGradGuard guard;
+      const auto dtype = weight.scalar_type();
+      if (gy.defined()) {
+        std::tie(gx, gw, gb) = act8_layer_norm_bwd(gy.to(dtype), gs.defined() ? maybe(gs.to(dtype)) : std::nullopt, q,
+                                                   scale, weight, mean, rstd, maybe(rows));
+      } else if (gs.defined()) {                 // only s was used: its gradient passes through
+        gx = gs.to(dtype);
+        gw = at::zeros_like(weight);
+        gb = at::zeros_like(weight);
+      }
+    }
+    variable_list out = once({gx, gw, gb});
+    return {out[0], residual ? out[0] : at::Tensor(), out[1], out[2], at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor layer_norm_act8(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps,
+                           const std::optional<at::Tensor>& rows, const std::optional<at::Tensor>& pad,
+                           int64_t out_rows) {
+  if (keeps({&x, &weight, &bias}))
+    return LayerNormAct8::apply(x, std::optional<at::Tensor>(), weight, bias, eps, rows, pad, out_rows)[0];
+  at::Tensor y = std::get<1>(act8_layer_norm_fwd(x, std::nullopt, weight, bias, eps, rows, out_rows, false));
+  clear_rows(y, pad);
+  return y;
+}
+
+std::tuple<at::Tensor, at::Tensor> add_layer_norm_act8(const at::Tensor& x, const at::Tensor& r,
+                                                       const at::Tensor& weight, const at::Tensor& bias, double eps,
+                                                       const std::optional<at::Tensor>& rows,
+                                                       const std::optional<at::Tensor>& pad, int64_t out_rows) {
+  if (keeps({&x, &r, &weight, &bias})) {
+    auto out = LayerNormAct8::apply(x, std::optional<at::Tensor>(r), weight, bias, eps, rows, pad, out_rows);
+    return {out[0], out[1]};
+  }
+  auto [s, y, q, scale, mean, rstd] = act8_layer_norm_fwd(x, r, weight, bias, eps, rows, out_rows, false);
+  clear_rows(y, pad);
+  return {s, y};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(visionseg, m) {
@@ -703,6 +823,12 @@ TORCH_LIBRARY(visionseg, m) {
         "Tensor rstd, Tensor? rows=None) -> (Tensor, Tensor, Tensor)");
   m.def("act8_wgrad(Tensor grad_y, Tensor q, Tensor scale, int features, ScalarType dtype, bool bias=False) "
         "-> (Tensor, Tensor)");
+  // with autograd (a function given here runs for every key: it takes its own gradient)
+  m.def("gelu_act8(Tensor x) -> Tensor", gelu_act8);
+  m.def("layer_norm_act8(Tensor x, Tensor weight, Tensor bias, float eps, Tensor? rows=None, Tensor? pad=None, "
+        "int out_rows=0) -> Tensor", layer_norm_act8);
+  m.def("add_layer_norm_act8(Tensor x, Tensor r, Tensor weight, Tensor bias, float eps, Tensor? rows=None, "
+        "Tensor? pad=None, int out_rows=0) -> (Tensor, Tensor)", add_layer_norm_act8);
 }
 
 TORCH_LIBRARY_IMPL(visionseg, CUDA, m) {

@@ -23,9 +23,9 @@ import os
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from .profiling import enabled as profiling_enabled
 from .profiling import timed
 
 
@@ -1550,19 +1550,42 @@ def activation(x, kind: str, gelu_sink=None):
 # `scale` uint8 [..., P / 32] = e + 127; a block with an infinity or a NaN (or a magnitude
 # above 127 * 2^121) is kept as NaN (scale 255).  The forward results are not touched: only the backward formulas are taken at the
 # checkpointed values.
+_ACT8 = None
+
+
+def _act8():
+    """The overloads of these ops in torch.ops.visionseg, looked up once."""
+    global _ACT8
+    if _ACT8 is None:
+        t = L.tops()
+        _ACT8 = {n: getattr(t, n).default for n in ("act8_pack", "act8_unpack", "act8_wgrad", "act8_gelu_fwd",
+                                                    "act8_gelu_bwd", "gelu_act8", "layer_norm_act8",
+                                                    "add_layer_norm_act8")}
+    return _ACT8
+
+
+def _act8_call(name, like, tensors, checkpoints, *args, flops=0):
+    """The op on args; its forward timed where a KernelTimer is active, as `tensors` passes over a
+    tensor like `like` and `checkpoints` over its checkpoint."""
+    op = _act8()[name]
+    if not profiling_enabled():
+        return op(*args)
+    n = like.numel()
+    with timed(name, like, bytes_=n * (tensors * like.element_size() + checkpoints), flops=float(n * flops)):
+        return op(*args)
+
+
 def act8_pack(x):
     """x [..., C] (f32 / bf16; a 2-D x may have any row stride) -> (q, scale)."""
     L.require_hip(x)
-    with timed("act8_pack", x, bytes_=x.numel() * (x.element_size() + 1)):
-        return L.tops().act8_pack(x)
+    return _act8_call("act8_pack", x, 1, 1, x)
 
 
 def act8_unpack(q, scale, features: int, dtype):
     """The values [..., features] that a checkpoint stands for, in dtype (f32 / bf16: both
     exact)."""
     L.require_hip(q, scale)
-    with timed("act8_unpack", q, bytes_=q.numel() * 3):
-        return L.tops().act8_unpack(q, scale, int(features), dtype)
+    return _act8_call("act8_unpack", q, 3, 0, q, scale, features, dtype)
 
 
 def act8_wgrad(gy, q, scale, features: int, out_dtype, bias: bool = False):
@@ -1571,94 +1594,35 @@ def act8_wgrad(gy, q, scale, features: int, out_dtype, bias: bool = False):
     (dW, db) with db [N] = the column sums of gy.  Exact products, f32 accumulation
     (csrc/act8_wgrad.hip; the uncompressed form is token_wgrad)."""
     L.require_hip(gy, q, scale)
-    with timed("act8_wgrad", gy, flops=2.0 * gy.numel() * features, bytes_=gy.numel() * gy.element_size() + q.numel()):
-        dw, db = L.tops().act8_wgrad(gy, q, scale, int(features), out_dtype, bool(bias))
+    dw, db = _act8_call("act8_wgrad", gy, 1, 0, gy, q, scale, features, out_dtype, bias, flops=2 * features)
     return (dw, db) if bias else dw
-
-
-def _keeps(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
-class GeluAct8Function(torch.autograd.Function):
-    """Exact GELU keeping its input as an 8-bit checkpoint."""
-
-    @staticmethod
-    def forward(ctx, x, keep):
-        with timed("gelu_act8_fwd", x, bytes_=x.numel() * (2 * x.element_size() + 1)):
-            y, q, scale = L.tops().act8_gelu_fwd(x, keep)
-        if keep:
-            ctx.save_for_backward(q, scale)
-            ctx.dtype = x.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        q, scale = ctx.saved_tensors
-        with timed("gelu_act8_bwd", gy, bytes_=gy.numel() * (2 * gy.element_size() + 1)):
-            gx, _ = L.tops().act8_gelu_bwd(gy.to(ctx.dtype), q, scale, False)
-        return gx, None
 
 
 def gelu_act8(x):
     """F.gelu(x) (exact) for x [..., C] f32 / bf16, whose backward reads x's 8-bit checkpoint
-    instead of x: dx = dy (Phi(h) + h phi(h)) at the checkpointed h."""
+    instead of x: dx = dy (Phi(h) + h phi(h)) at the checkpointed h (once differentiable)."""
     L.require_hip(x)
-    return GeluAct8Function.apply(x, _keeps(x))
-
-
-class LayerNormAct8Function(torch.autograd.Function):
-    """layer_norm keeping the normalised tensor as an 8-bit checkpoint (csrc/act8_norm.hip)."""
-
-    @staticmethod
-    def forward(ctx, x, r, weight, bias, eps, wrows, keep):
-        ctx.set_materialize_grads(False)
-        n = x.numel()
-        with timed("layer_norm_act8_fwd", x, bytes_=n * ((2 if r is None else 4) * x.element_size() + 1)):
-            s, y, q, scale, mean, rstd = L.tops().act8_layer_norm_fwd(
-                x, r, weight, bias, float(eps), wrows.rows if wrows is not None else None,
-                wrows.total if wrows is not None else 0, keep)
-        if wrows is not None and wrows.pad.numel():
-            y.index_fill_(0, wrows.pad, 0)
-        if keep:
-            ctx.save_for_backward(q, scale, weight, mean, rstd)
-            ctx.wrows = wrows
-        return y if r is None else (s, y)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        q, scale, weight, mean, rstd = ctx.saved_tensors
-        gs, gy = (None, grads[0]) if len(grads) == 1 else grads
-        dt, C = weight.dtype, weight.numel()
-        lead = q.shape[:-1]
-        if gy is None:                  # only s was used: its gradient passes through
-            gw = torch.zeros_like(weight) if ctx.needs_input_grad[2] else None
-            return (gs, gs if ctx.needs_input_grad[1] else None, gw,
-                    torch.zeros_like(weight) if ctx.needs_input_grad[3] else None, None, None, None)
-        n = gy.numel()
-        with timed("layer_norm_act8_bwd", gy, bytes_=n * ((2 if gs is None else 3) * gy.element_size() + 1)):
-            gx, gw, gb = L.tops().act8_layer_norm_bwd(
-                gy.to(dt), gs.to(dt) if gs is not None else None, q, scale, weight, mean, rstd,
-                ctx.wrows.rows if ctx.wrows is not None else None)
-        gx = gx.view(*lead, C)
-        return gx, gx if ctx.needs_input_grad[1] else None, gw, gb, None, None, None
+    return _act8_call("gelu_act8", x, 2, 1, x)
 
 
 def layer_norm_act8(x, weight, bias, eps: float = 1e-5, wrows=None):
     """layer_norm (x [..., C], C <= 8192; weight and bias [C] in x's dtype, f32 / bf16) whose
     backward reads x's 8-bit checkpoint instead of x: xh = (h - mean) rstd with x's own mean and
-    rstd.  `wrows`: y in the window layout (see LayerNormFunction)."""
+    rstd (csrc/act8_norm.hip; once differentiable).  `wrows`: y in the window layout (see
+    LayerNormFunction)."""
     L.require_hip(x, weight, bias)
-    return LayerNormAct8Function.apply(x, None, weight, bias, eps, wrows, _keeps(x, weight, bias))
+    if wrows is None:
+        return _act8_call("layer_norm_act8", x, 2, 1, x, weight, bias, eps)
+    return _act8_call("layer_norm_act8", x, 2, 1, x, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
 
 
 def add_layer_norm_act8(x, r, weight, bias, eps: float = 1e-5, wrows=None):
     """add_layer_norm -- (s, layer_norm(s)) with s = x + r -- keeping s as an 8-bit checkpoint
     (see layer_norm_act8)."""
     L.require_hip(x, r, weight, bias)
-    return LayerNormAct8Function.apply(x, r, weight, bias, eps, wrows, _keeps(x, r, weight, bias))
+    if wrows is None:
+        return _act8_call("add_layer_norm_act8", x, 4, 1, x, r, weight, bias, eps)
+    return _act8_call("add_layer_norm_act8", x, 4, 1, x, r, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
 
 
 # ------------------------------------------------------------------ per-parameter clip
