@@ -84,6 +84,8 @@ def parse():
                     help="C5: Swin window attention on fp8 (e4m3) MFMA (window^2 <= 160; bf16 elsewhere)")
     ap.add_argument("--linear-fp8", action="store_true",
                     help="C5: the Swin blocks' K-deep Linears on the block-scaled MX fp8 MFMA (csrc/token_gemm.hip)")
+    ap.add_argument("--act8", action="store_true",
+                    help="8-bit activation checkpoints in the Swin blocks (M2FConfig.act8)")
     ap.add_argument("--no-parity", action="store_true")
     ap.add_argument("--arch", default="mask2former", choices=["mask2former", "maskdino"],
                     help="mask2former (C1-C3, C5) or maskdino (C4: 300 queries, 4-level encoder, DN; parity unpinned)")
@@ -360,11 +362,12 @@ def main():
         from visionseg.maskdino import MaskDINO, MaskDINOConfig, MaskDINOCriterion
         if a.queries == 100:
             a.queries = 300
-        cfg = MaskDINOConfig.preset(a.model, num_queries=a.queries)
+        cfg = MaskDINOConfig.preset(a.model, num_queries=a.queries, act8=a.act8)
         model = MaskDINO(cfg).init_weights(seed=0)
         crit = MaskDINOCriterion(cfg, matcher=a.matcher)
     else:
-        cfg = M2FConfig.preset(a.model, num_queries=a.queries, attn_fp8=a.attn_fp8, linear_fp8=a.linear_fp8)
+        cfg = M2FConfig.preset(a.model, num_queries=a.queries, attn_fp8=a.attn_fp8, linear_fp8=a.linear_fp8,
+                               act8=a.act8)
         model = Mask2Former(cfg).init_weights(seed=0)
         crit = SetCriterion(cfg, matcher=a.matcher)
     trainer = Trainer(model, crit, SolverConfig(precision=a.precision, optimizer=a.optimizer), device=dev,
@@ -438,7 +441,8 @@ def main():
             "config": {"workload": f"{_config_tag(a.model, a.size, a.arch, a.attn_fp8 or a.linear_fp8)}: {a.model} + {a.arch}, "
                                    f"{a.batch}x3x{a.size}^2 per GPU, {cfg.num_queries} queries, {prec}"
                                    f"{', fp8 (e4m3) window attention' if a.attn_fp8 else ''}"
-                                   f"{', MX-fp8 (e4m3 + e8m0 per 32) Swin Linears with K >= 384' if a.linear_fp8 else ''}, 1 class",
+                                   f"{', MX-fp8 (e4m3 + e8m0 per 32) Swin Linears with K >= 384' if a.linear_fp8 else ''}"
+                                   f"{', 8-bit activation checkpoints in the Swin blocks' if a.act8 else ''}, 1 class",
                        "model": f"{a.model}_{a.arch}", "global_batch": a.batch * world, "image_size": a.size,
                        "parallelism": f"dp{world}"},
             "final_loss": round(float(loss.item()), 4),

@@ -542,6 +542,50 @@ def test_swin_backbone(dtype):
     assert out[True][2] < 0.75 * out[False][2], (out[True][2], out[False][2])
 
 
+def test_trainer():
+    """Training steps of the whole model under M2FConfig.act8, replayed as HIP graphs and eager: the
+    same losses and weights, to the noise of the float atomics elsewhere in the model (the bounds of
+    tests/test_gpu_graphs.py)."""
+    import copy
+    from test_gpu_graphs import _compare, _run
+    from visionseg.criterion import SetCriterion
+    from visionseg.data import synthetic_batch
+    from visionseg.model import M2FConfig, Mask2Former
+    from visionseg.train import Trainer
+    dev = torch.device(DEV, 0)
+    cfg = M2FConfig.preset("swin_t", num_queries=20, act8=True)
+    model = Mask2Former(cfg).init_weights(seed=0)
+    batch = synthetic_batch(2, 256, seed=1, device=dev)
+    ta = Trainer(copy.deepcopy(model), SetCriterion(cfg), device=dev)
+    tb = Trainer(copy.deepcopy(model), SetCriterion(cfg), device=dev, graphs=True, graph_warmup=2)
+    la, lb = _run(ta, [batch] * 6), _run(tb, [batch] * 6)
+    assert tb.captures == 1
+    _compare(ta, tb, la, lb)
+
+
+def test_predictor_and_checkpoints():
+    """Without gradients the act8 model keeps nothing and predicts what it does in training; its
+    state dict is the plain model's."""
+    from visionseg.model import M2FConfig, Mask2Former
+    kw = dict(embed_dim=32, depths=(2, 2, 2, 2), num_heads=(1, 2, 4, 8), feature_size=64, mask_feature_size=64,
+              hidden_dim=64, enc_ffn=128, dec_ffn=128, dec_heads=2, enc_layers=2, dec_layers=4, num_queries=10)
+    torch.manual_seed(4)
+    plain, packed = Mask2Former(M2FConfig(**kw)), Mask2Former(M2FConfig(act8=True, **kw))
+    packed.load_state_dict(plain.state_dict())
+    plain, packed = plain.to(DEV), packed.to(DEV)
+    im = torch.randn(1, 3, 128, 160, generator=_gen(1), device=DEV)
+    with torch.no_grad():
+        a, b = plain.backbone(im), packed.backbone(im)
+        kept = packed.backbone(im)
+    for x, y, z in zip(a, b, kept):
+        assert torch.equal(y, z)
+        assert float((x - y).norm() / x.norm()) < 1e-5
+    with torch.enable_grad():
+        for y, z in zip(b, packed.backbone(im)):
+            # (the Linears of training and inference may be different GEMMs)
+            assert float((y - z.detach()).norm() / y.norm()) < 1e-5
+
+
 def test_on_another_stream():
     ops = _ops()
     side = torch.cuda.Stream()

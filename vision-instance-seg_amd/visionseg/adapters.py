@@ -91,13 +91,14 @@ def train_mask2former(exp_name, train_dir, test_dir, output_dir, hyperparams, ba
         pad_buckets = default_pad_buckets(min_sizes, max_size)
     ds = CocoInstanceDataset(str(train_dir), min_size=min_sizes, max_size=max_size, train=True, seed=seed + rank)
     backbone = str(hp.get("backbone", backbone))
+    act8 = bool(hp.get("act8", False))                # 8-bit activation checkpoints in the backbone (M2FConfig.act8)
     if arch == "maskdino":
         from .maskdino import MaskDINO, MaskDINOConfig, MaskDINOCriterion
-        cfg = MaskDINOConfig.preset(backbone, num_labels=max(1, len(ds.cat_to_label)))
+        cfg = MaskDINOConfig.preset(backbone, num_labels=max(1, len(ds.cat_to_label)), act8=act8)
         model = MaskDINO(cfg).init_weights(seed)
         criterion = MaskDINOCriterion(cfg)
     else:
-        cfg = M2FConfig.preset(backbone, num_labels=max(1, len(ds.cat_to_label)))
+        cfg = M2FConfig.preset(backbone, num_labels=max(1, len(ds.cat_to_label)), act8=act8)
         model = Mask2Former(cfg).init_weights(seed)
         criterion = SetCriterion(cfg)
     bs = int(hp["batch_size"])
