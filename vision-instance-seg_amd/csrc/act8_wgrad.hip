@@ -7,8 +7,8 @@
 // way into LDS, once a workgroup, exactly (act8.h).  f32 gradients are cut into three bf16 parts
 // by truncation, gY = hi + mid + lo: 8 bits of significand each, so the sum is exact, and three
 // matrix products give what an f32 product of exact terms would; a non-finite value is its hi
-// part alone.  Accumulation is f32 in the matrix units.  db is summed on the way into LDS by the
-// workgroups of the first input columns.
+// part alone.  Accumulation is f32 in the matrix units.  db is summed on the way into LDS, every
+// workgroup of an output block its share of the chunks.
 //
 // A workgroup owns BO output rows x BI input columns of dW for one split of the tokens.  LDS holds
 // two chunks: while chunk c is multiplied, chunk c + 1 goes from registers into LDS and chunk
@@ -29,7 +29,7 @@ struct Wgrad8 {
   void* dw;
   void* db;
   float* part;                                   // [S][tiles][BO * BI] in fragment order (S > 1)
-  float* pbias;                                  // [S][N]
+  float* pbias;                                  // [S][tiles_i][N]
   long long ldg, T;
   int N, K, P;                                   // P: the checkpoint's pitch
   int S, tiles_i, tiles;
@@ -92,6 +92,14 @@ __device__ __forceinline__ void lds16(lds_byte* p, uint4 a) {
   *(__attribute__((address_space(3))) u32x4*)p = v;
 }
 
+// Byte offset of (row, 16-B column) in an image of h.  A thread writes two neighbouring columns, 2 x
+// and 2 x + 1, one after the other: the even columns are stored in front of the odd ones, so that
+// eight lanes write 128 B of different banks.  The four rows x four columns that a transposing
+// read takes at a time lie in 16 different places of 256 B, by the exclusive or with the row.
+__device__ __forceinline__ int xoff16(int row, int col) {
+  return 256 * row + 16 * (((col >> 1) | ((col & 1) << 3)) ^ ((row & 3) << 1));
+}
+
 // acc += h^T gY over the wave's TO x TI tiles of 32 x 32, chunk by chunk
 template <typename T, int BO, int BI, int WO, int WI, int TK, bool FAST>
 __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a) {
@@ -113,7 +121,6 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   const int wo = qo * (BO / WO), wi = qi * (BI / WI);
   const int nchunk = (int)((a.T + TK - 1) / TK);
   const int cb = (int)((long long)nchunk * s / a.S), ce = (int)((long long)nchunk * (s + 1) / a.S);
-  const bool do_bias = a.db != nullptr && ib == 0;
 
   const int gr = threadIdx.x / GC, gc = threadIdx.x % GC, xr = threadIdx.x / XC, xc = threadIdx.x % XC;
   const int gcol = ob * BO + gc * 8, xcol = ib * BI + xc * 16;
@@ -178,13 +185,9 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   lds_byte* at_g[GD];
 #pragma unroll
   for (int d = 0; d < GD; ++d) at_g[d] = base + (gc >> 4) * kImg + woff(gr + d * (NT / GC), gc & 15);
-  // four neighbouring lanes write the first 16-B half of their pieces of q first, the next four the
-  // second: eight lanes then cover 128 B of banks
-  const bool swap = (xc >> 2) & 1;
   lds_byte* at_x[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    at_x[h] = base + (NP * NHO + (xc >> 3)) * kImg + woff(xr, 2 * (xc & 7) + ((h == 1) != swap ? 1 : 0));
+  for (int h = 0; h < 2; ++h) at_x[h] = base + (NP * NHO + (xc >> 3)) * kImg + xoff16(xr, 2 * (xc & 7) + h);
   lds_byte *at_b[TO][2], *at_a[TI][2];
   {
     const int row = 8 * hh + ((l & 15) >> 2), col = (l & 16) + 4 * (l & 3);
@@ -198,40 +201,47 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
 #pragma unroll
       for (int ti = 0; ti < TI; ++ti) {
         const int c = ((wi + 32 * ti) & 127) + col;
-        at_a[ti][h] = base + (NP * NHO + ((wi + 32 * ti) >> 7)) * kImg + woff(row + 4 * h, c >> 3) + (c & 7) * 2;
+        at_a[ti][h] = base + (NP * NHO + ((wi + 32 * ti) >> 7)) * kImg + xoff16(row + 4 * h, c >> 3) + (c & 7) * 2;
       }
     }
   }
-  float bsum[8];                                 // this thread's columns of gY, summed as they pass
+  // db: this thread's columns of gY, summed as they pass.  The workgroups of an output block share a
+  // split's chunks, this one's are [b0, b1); the first workgroup has them all where there is no
+  // second kernel to add them up, and on the largest tile, which has no registers for a third loop
+  // (47 us against 51 at 262144 x 96 x 384 on the smallest tile; 592 against 585 at 147456 x 1024 x
+  // 2048 on the largest)
+  constexpr bool SHARE = TO * TI < 8;
+  const int shares = SHARE && a.S > 1 ? a.tiles_i : 1;
+  const bool do_bias = a.db != nullptr && ib < shares;
+  const int b0 = do_bias ? cb + (int)((long long)(ce - cb) * ib / shares) : cb;
+  const int b1 = do_bias ? cb + (int)((long long)(ce - cb) * (ib + 1) / shares) : cb;
+  float bsum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) bsum[i] = 0.f;
   auto put_g = [&](int p, auto bias_tag) {
     constexpr bool BIAS = decltype(bias_tag)::value;
     lds_byte* to = at_g[p % GD] + (p / GD) * GD * (NT / GC) * 256;
-    if constexpr (NP == 3 || BIAS) {
-      float v[8];
-      g[p].unpack(v);
-      if constexpr (BIAS) {
+    float v[8];
+    if constexpr (NP == 3 || BIAS) g[p].unpack(v);
+    if constexpr (BIAS) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bsum[i] += v[i];
-      }
-      if constexpr (NP == 3) {
-        uint4 hi, mid, lo;
-        split3(v, hi, mid, lo);
-        lds16(to, hi);
-        lds16(to + NHO * kImg, mid);
-        lds16(to + 2 * NHO * kImg, lo);
-      }
+      for (int i = 0; i < 8; ++i) bsum[i] += v[i];
     }
-    if constexpr (NP == 1) lds16(to, g[p].a);
+    if constexpr (NP == 3) {
+      uint4 hi, mid, lo;
+      split3(v, hi, mid, lo);
+      lds16(to, hi);
+      lds16(to + NHO * kImg, mid);
+      lds16(to + 2 * NHO * kImg, lo);
+    } else {
+      lds16(to, g[p].a);
+    }
   };
   auto put_x = [&](int p) {
-    const uint2 lo = make_uint2(xq[p].x, xq[p].y), hi = make_uint2(xq[p].z, xq[p].w);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[8];
-      const bool second = (h == 1) != swap;
-      unpack_chunk(make_uint2(second ? hi.x : lo.x, second ? hi.y : lo.y), xs[p], v);
+      unpack_chunk(h == 0 ? make_uint2(xq[p].x, xq[p].y) : make_uint2(xq[p].z, xq[p].w), xs[p], v);
       uint32_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)                // exact in bf16: the upper halves
@@ -252,13 +262,20 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
 #pragma unroll
     for (int y = 0; y < TI; ++y) zero16(acc[x][y]);
 
-  auto run = [&](auto bias_tag) {
+  // MODE 0: no db, 1: db from every chunk, 2: from [b0, b1)
+  auto run = [&](auto mode_tag) {
+    constexpr int MODE = decltype(mode_tag)::value;
     // the first chunk into LDS, the next one into the registers
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (j == 1) {
+        if (MODE == 1 || (MODE == 2 && b0 == cb && b1 > cb)) {
 #pragma unroll
-        for (int p = 0; p < GP; ++p) put_g(p, bias_tag);
+          for (int p = 0; p < GP; ++p) put_g(p, std::true_type{});
+        } else {
+#pragma unroll
+          for (int p = 0; p < GP; ++p) put_g(p, std::false_type{});
+        }
 #pragma unroll
         for (int p = 0; p < XP; ++p) put_x(p);
         to_stage(1);
@@ -297,7 +314,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
     static_assert(KS % 2 == 0, "the operands' two sets alternate over chunks");
     int flip = 1;                                // from the stage that is read to the other one
     read(0, 0);
-    for (int c = cb; c < ce; ++c) {
+    auto chunk = [&](auto bias_tag) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         if (k + 1 < KS) {
@@ -307,12 +324,12 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
           // it visible and its own place free, with the last step's MFMAs still to issue
           if constexpr (TO * TI >= 8) {
             // the steps before, MFMA by MFMA with a share of the operand reads and of the pieces'
-            // arithmetic behind each (1257 ns a chunk against 1374 as the compiler has it, and 44
-            // against 45 us at 16384 x 1536 x 384; the smaller tiles lose by it)
+            // arithmetic behind each (alone on the chip 1257 ns a chunk against 1374 as the compiler
+            // has it; the smaller tiles lose by it)
 #pragma unroll
             for (int i = 0; i < (KS - 1) * TO * TI; ++i) {
               __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);      // MFMA
-              __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);      // vector arithmetic
+              __builtin_amdgcn_sched_group_barrier(0x2, decltype(bias_tag)::value ? 5 : 3, 0);      // vector arithmetic
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);    // LDS reads
             }
           }
@@ -343,14 +360,23 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
       advance();
       to_stage(-flip);
       flip = -flip;
+    };
+    // (at chunk c, chunk c + 1 passes through the registers)
+    int c = cb;
+    if constexpr (MODE == 2) {
+      for (; c < b0 - 1; ++c) chunk(std::false_type{});
+      for (; c < b1 - 1; ++c) chunk(std::true_type{});
     }
+    for (; c < ce; ++c) chunk(std::integral_constant<bool, MODE == 1>{});
     lds_barrier();
   };
-  if (do_bias)
-    run(std::true_type{});
+  if constexpr (SHARE)
+    run(std::integral_constant<int, 2>{});
+  else if (do_bias)
+    run(std::integral_constant<int, 1>{});
   else
-    run(std::false_type{});
-  if (do_bias) {                                 // the threads that hold the same columns, in order
+    run(std::integral_constant<int, 0>{});
+  if (do_bias) {          // the threads that hold the same columns, in order
     float* sum = reinterpret_cast<float*>(smem);
     constexpr int R = NT / GC;
 #pragma unroll
@@ -362,7 +388,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
 #pragma unroll
       for (int k = 0; k < R; ++k) t += sum[k * BO + threadIdx.x];
       if (a.S > 1)
-        a.pbias[(size_t)s * a.N + o] = t;
+        a.pbias[((size_t)s * shares + ib) * a.N + o] = t;
       else
         store_out(a.db, o, a.f32_out, t);
     }
@@ -398,7 +424,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
 // dW = the splits' partials added in order, in the partials' own order: a wave reads 1 KB (the
 // 32 x 8 values of a register group) of each split at a time.  A workgroup takes 64 float4 in
 // NG interleaved slices of the splits, whose sums it adds in order; the workgroups behind dW's
-// do the same for db.
+// are db's.
 template <int BO, int BI, int WO, int WI, int NG>
 __global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a) {
   constexpr int TO = BO / WO / 32, TI = BI / WI / 32, GROUPS = BO * BI / 256;
@@ -406,16 +432,21 @@ __global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a)
   const int l = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const long long n = (long long)a.tiles * GROUPS;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (blockIdx.x >= n) {
-    const long long o = (blockIdx.x - n) * 64 + l;
-    if (o < a.N)
-      for (int s = sl; s < a.S; s += NG) v.x += a.pbias[(size_t)s * a.N + o];
-    lds[sl][l] = v;
+  if (blockIdx.x >= n) {                         // db: 16 columns x 4 NG slices of the partial rows
+    float* sum = reinterpret_cast<float*>(&lds[0][0]);
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const long long o = (blockIdx.x - n) * 16 + col;
+    const int rows = a.S * (TO * TI < 8 ? a.tiles_i : 1);      // (SHARE)
+    float t = 0.f;
+    if (o < a.N) {
+#pragma unroll 8
+      for (int s = slice; s < rows; s += 4 * NG) t += a.pbias[(size_t)s * a.N + o];
+    }
+    sum[slice * 16 + col] = t;
     __syncthreads();
-    if (sl == 0 && o < a.N) {
-      float t = v.x;
+    if (slice == 0 && o < a.N) {
 #pragma unroll
-      for (int k = 1; k < NG; ++k) t += lds[k][l].x;
+      for (int k = 1; k < 4 * NG; ++k) t += sum[k * 16 + col];
       store_out(a.db, o, a.f32_out, t);
     }
     return;
@@ -502,8 +533,8 @@ bool sizes_ok(long long T, int N, int K) {
          (long long)((N + 127) / 128) * ((K + 127) / 128) < (1 << 20);
 }
 
-long long workspace_bytes(const Plan& p, int N) {
-  return p.S == 1 ? 0 : 4ll * p.S * (p.tiles * p.bo * p.bi + N);
+long long workspace_bytes(const Plan& p, int N, int K) {
+  return p.S == 1 ? 0 : 4ll * p.S * (p.tiles * p.bo * p.bi + (long long)((K + p.bi - 1) / p.bi) * N);
 }
 
 template <typename T, int BO, int BI, int WO, int WI, int TK>
@@ -518,7 +549,7 @@ int launch(const Wgrad8& a, bool fast, hipStream_t st) {
   VS_LAUNCH_CHECK();
   if (a.S > 1) {
     constexpr int NG = 4;
-    const long long groups = (long long)a.tiles * (BO * BI / 256) + (a.db ? (a.N + 63) / 64 : 0);
+    const long long groups = (long long)a.tiles * (BO * BI / 256) + (a.db ? (a.N + 15) / 16 : 0);
     hipLaunchKernelGGL((act8_wgrad_sum_kernel<BO, BI, WO, WI, NG>), dim3((unsigned)groups), dim3(64 * NG), 0, st, a);
     VS_LAUNCH_CHECK();
   }
@@ -532,7 +563,7 @@ using namespace vs;
 
 extern "C" long long vs_act8_wgrad_workspace_bytes(int dtype, long long tokens, int N, int K) {
   if (!sizes_ok(tokens, N, K) || N == 0 || K == 0) return 0;
-  return workspace_bytes(plan_of(dtype == VS_F32, tokens, N, K), N);
+  return workspace_bytes(plan_of(dtype == VS_F32, tokens, N, K), N, K);
 }
 
 extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long ld_gy, const void* q,
