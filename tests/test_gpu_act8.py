@@ -586,6 +586,55 @@ def test_predictor_and_checkpoints():
             assert float((y - z.detach()).norm() / y.norm()) < 1e-5
 
 
+def test_inference_mode_and_one_dimension():
+    ops = _ops()
+    x = _act(5, 40, F32, 1)
+    w, b = torch.rand(40, device=DEV).requires_grad_(), torch.rand(40, device=DEV).requires_grad_()
+    want = ops.layer_norm_act8(x, w, b).detach(), ops.gelu_act8(x)
+    with torch.inference_mode():
+        assert torch.equal(ops.layer_norm_act8(x, w, b), want[0]) and torch.equal(ops.gelu_act8(x), want[1])
+        assert torch.equal(ops.add_layer_norm_act8(x, x, w, b)[0], 2 * x)
+    # one row without a dimension for it: the same as a matrix of one row
+    assert torch.equal(ops.gelu_act8(x[1]), want[1][1]) and torch.equal(ops.layer_norm_act8(x[1], w, b), want[0][1])
+    q, s = ops.act8_pack(x[1])
+    assert torch.equal(ops.act8_unpack(q, s, 40, F32), ops.act8_unpack(*ops.act8_pack(x), 40, F32)[1])
+    gy = _grad(5, 24, F32, 2)
+    assert torch.equal(ops.act8_wgrad(gy[1], q, s, 40, F32), ops.act8_wgrad(gy[1:2], q[None], s[None], 40, F32))
+
+
+def test_whole_gradients_by_expansion():
+    """The gradient that sum() sends back is one number without strides."""
+    ops = _ops()
+    x = _act(6, 40, F32, 1).requires_grad_()
+    w, b = torch.rand(40, device=DEV).requires_grad_(), torch.rand(40, device=DEV).requires_grad_()
+    for f, ts in ((lambda: ops.gelu_act8(x), (x,)), (lambda: ops.layer_norm_act8(x, w, b), (x, w, b))):
+        a = torch.autograd.grad(f().sum(), ts)
+        y = f()
+        c = torch.autograd.grad(y, ts, torch.ones_like(y))
+        assert all(torch.equal(p, q) for p, q in zip(a, c))
+    q, s = ops.act8_pack(x.detach())
+    one = torch.ones((), device=DEV).expand(6, 24)
+    dw, db = ops.act8_wgrad(one, q, s, 40, F32, bias=True)
+    dw0, db0 = ops.act8_wgrad(one.contiguous(), q, s, 40, F32, bias=True)
+    assert torch.equal(dw, dw0) and torch.equal(db, db0)
+
+
+def test_two_streams_at_once():
+    ops = _ops()
+    sets = [(_act(20000, 256, BF16, k), _grad(20000, 256, BF16, 10 + k)) for k in range(2)]
+    want = [ops.act8_wgrad(gy, *ops.act8_pack(x), 256, F32, bias=True) for x, gy in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for st, (x, gy) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(ops.act8_wgrad(gy, *ops.act8_pack(x), 256, F32, bias=True))
+        torch.cuda.synchronize()
+        for (a, b), (c, d) in zip(got, want):
+            assert torch.equal(a, c) and torch.equal(b, d)
+
+
 def test_on_another_stream():
     ops = _ops()
     side = torch.cuda.Stream()

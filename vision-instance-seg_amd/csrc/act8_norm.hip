@@ -12,6 +12,9 @@
 // more than 2048 features take the whole workgroup (G = 256, one exchange through LDS).
 // Statistics are f32, the variance in a second pass over the registers.
 //
+// Measured: 589824 x 192 bf16 with the residual, forward 192 us (5.3 TB/s), backward 166 (4.8) + 5 for
+// the sum;  65536 x 768 bf16, 41 (6.1) and 51 (4.9);  4099 x 1003 f32, 10 (3.7) and 13 + 3.6 (2.8).
+//
 // dw / db: summed by every lane over the rows it sweeps, over the workgroup's groups in LDS,
 // written as one f32 row a workgroup and added up by a second kernel: a fixed order, no atomics.
 #include <type_traits>
@@ -258,7 +261,9 @@ __global__ void __launch_bounds__(1024) act8_ln_sum_kernel(const float* __restri
 
 // calls go(G, K) (integral constants) for the lanes a row and chunks a lane of C features: the
 // fewest lanes (4, 8, ... 64) that hold the row in at most three chunks each -- 96, 192, 384, ...
-// features then fill every lane -- else up to four, else the workgroup
+// features then fill every lane -- else up to four, else the workgroup.  (Forward / backward us with
+// at most three, two, one chunk a lane: 589824 x 192 with the residual 203 / 158, 208 / 179, 229 /
+// 156;  65536 x 768 41 / 51, 43 / 51, 90 / 84.)
 template <typename F>
 void with_shape(int C, F&& go) {
   using std::integral_constant;

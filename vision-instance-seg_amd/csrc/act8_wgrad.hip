@@ -14,6 +14,18 @@
 // two chunks: while chunk c is multiplied, chunk c + 1 goes from registers into LDS and chunk
 // c + 2 from memory into the registers, piece by piece between the MFMAs; one barrier a chunk.
 // Splits write f32 partials that a second kernel adds up in a fixed order (no atomics).
+//
+// What bounds it.  Vector arithmetic costs MFMA time almost in full (64 idle instructions more a
+// chunk: 10 to 16 % more time), so the widening of the checkpoint, 2.5 instructions an element, is
+// what an uncompressed operand would save; at large sizes the clock falls to ~1.6 GHz with the matrix
+// units busy 68 % of the cycles.  Measured: 147456 tokens x 1024 x 2048 bf16 540-595 us (1040-1145
+// TF/s; the library's 8192^3 product 1475, its product at these sizes and layouts 570);  16384 x
+// 1536 x 384 35.8 us, of it 7.7 for the sum of 14 splits (33 MB of partials; the products alone are
+// 13 us at the library's rate);  262144 x 96 x 384 47.5;  400 x 256 x 256 9.5 (seven chunks in a
+// row: latency);  f32 10007 x 299 x 203 17.5 + 4.
+// Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
+// chunks in flight in registers (the loads are not what it waits for), a 128 x 128 tile a wave (four
+// waves of 256 x 256: spills).
 #include <type_traits>
 
 #include "act8.h"

@@ -1033,8 +1033,9 @@ class _MlpAct8Fn(torch.autograd.Function):
         h, hq, hs = ops._act8()["act8_gelu_fwd"](_forward_gemm(x, w1, b1).reshape(-1, w1.shape[0]), True)
         ctx.save_for_backward(q, scale, hq, hs, w1, w2)
         ctx.shape, ctx.has_bias = x.shape, (b1 is not None, b2 is not None)
-        T = h.shape[0]
-        ctx.wt = [_WT.request(w) if _dgrad_on_token_gemm(T, w, x.dtype) else None for w in (w1, w2)]
+        T, need = h.shape[0], ctx.needs_input_grad
+        ctx.wt = [_WT.request(w) if used and _dgrad_on_token_gemm(T, w, x.dtype) else None
+                  for w, used in ((w1, need[0]), (w2, True))]
         return _forward_gemm(h, w2, b2).view(*x.shape[:-1], w2.shape[0])
 
     @staticmethod
