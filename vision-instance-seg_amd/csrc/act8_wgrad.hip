@@ -73,21 +73,21 @@ __device__ __forceinline__ void store_four(const Wgrad8& a, int o, int i, float 
     if (i + e < a.K) store_out(a.dw, at + e, a.f32_out, v[e]);
 }
 
-// the bf16 parts of 8 f32 values (truncation; see the head of the file)
+// The bf16 parts of 8 f32 values (truncation; see the head of the file).  The rest of an infinity is
+// taken as 0, so that it stays one; that of a NaN is a NaN, also where truncation makes its hi part an
+// infinity.
 __device__ __forceinline__ void split3(const float* v, uint4& hi, uint4& mid, uint4& lo) {
-  uint32_t h[8], m[8], l[8];
+  float m[8], l[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t u = __float_as_uint(v[i]);
-    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-    h[i] = u & 0xffff0000u;
-    const float r1 = fin ? v[i] - __uint_as_float(h[i]) : 0.f;
-    m[i] = __float_as_uint(r1) & 0xffff0000u;
-    l[i] = __float_as_uint(r1 - __uint_as_float(m[i]));
-    if (!fin && (u & 0x7fffffu)) h[i] = 0x7fc00000u;          // a NaN whose payload is in the low bits
+    const float rest = __builtin_isinf(v[i]) ? 0.f : v[i] - __uint_as_float(__float_as_uint(v[i]) & 0xffff0000u);
+    m[i] = rest;
+    l[i] = rest - __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
   }
-  auto two = [](const uint32_t* w, int i) { return (w[i + 1] & 0xffff0000u) | (w[i] >> 16); };
-  hi = make_uint4(two(h, 0), two(h, 2), two(h, 4), two(h, 6));
+  auto two = [](const float* w, int i) {         // the upper halves of two values
+    return __builtin_amdgcn_perm(__float_as_uint(w[i + 1]), __float_as_uint(w[i]), 0x07060302u);
+  };
+  hi = make_uint4(two(v, 0), two(v, 2), two(v, 4), two(v, 6));
   mid = make_uint4(two(m, 0), two(m, 2), two(m, 4), two(m, 6));
   lo = make_uint4(two(l, 0), two(l, 2), two(l, 4), two(l, 6));
 }
