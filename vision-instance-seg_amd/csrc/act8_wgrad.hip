@@ -22,7 +22,8 @@
 // TF/s; the library's 8192^3 product 1475, its product at these sizes and layouts 570);  16384 x
 // 1536 x 384 35.8 us, of it 7.7 for the sum of 14 splits (33 MB of partials; the products alone are
 // 13 us at the library's rate);  262144 x 96 x 384 47.5;  400 x 256 x 256 9.5 (seven chunks in a
-// row: latency);  f32 10007 x 299 x 203 17.5 + 4.
+// row: latency);  f32 65536 x 768 x 768 208
+// (372 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 17.5 + 4.
 // Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
 // chunks in flight in registers (the loads are not what it waits for), a 128 x 128 tile a wave (four
 // waves of 256 x 256: spills).
@@ -191,12 +192,9 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   // LDS addresses, all of the current stage: the pieces' places (a piece's rows are 16 apart or a
   // multiple: the swizzle is the same) and the operands' (tr_frag: rows k.., 4 rows on, columns)
   typedef __attribute__((address_space(3))) bf16x4v_t lds_v4;
-  constexpr int GD = (NT / GC) % 16 == 0 ? 1 : 2;
-  static_assert((NT / GC) * GD % 16 == 0 && (NT / XC) % 16 == 0, "a thread's pieces have one swizzle");
+  static_assert((NT / GC) % 16 == 0 && (NT / XC) % 16 == 0, "a thread's pieces have one swizzle");
   lds_byte* const base = (lds_byte*)smem;
-  lds_byte* at_g[GD];
-#pragma unroll
-  for (int d = 0; d < GD; ++d) at_g[d] = base + (gc >> 4) * kImg + woff(gr + d * (NT / GC), gc & 15);
+  lds_byte* at_g = base + (gc >> 4) * kImg + woff(gr, gc & 15);
   lds_byte* at_x[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) at_x[h] = base + (NP * NHO + (xc >> 3)) * kImg + xoff16(xr, 2 * (xc & 7) + h);
@@ -232,7 +230,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   for (int i = 0; i < 8; ++i) bsum[i] = 0.f;
   auto put_g = [&](int p, auto bias_tag) {
     constexpr bool BIAS = decltype(bias_tag)::value;
-    lds_byte* to = at_g[p % GD] + (p / GD) * GD * (NT / GC) * 256;
+    lds_byte* to = at_g + p * (NT / GC) * 256;
     float v[8];
     if constexpr (NP == 3 || BIAS) g[p].unpack(v);
     if constexpr (BIAS) {
@@ -262,8 +260,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
     }
   };
   auto to_stage = [&](int step) {                // where the pieces go, `step` stages on
-#pragma unroll
-    for (int d = 0; d < GD; ++d) at_g[d] += step * kStage;
+    at_g += step * kStage;
     at_x[0] += step * kStage;
     at_x[1] += step * kStage;
   };
@@ -502,14 +499,15 @@ __global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a)
 // quarter, ... of them).  Measured as tile 0 / 1 / 2, us:  147456 tokens x 1024 x 2048: 635 / 677 /
 // 790;  65536 x 768 x 192: 48 / 42 / 52;  16384 x 1536 x 384: 45 / 37 / 41;  262144 x 96 x 384: 79 /
 // 67 / 52;  400 x 256 x 256: 20 / 13 / 9.5 (12 in two splits).  f32, tile 3 / 4: 65536 x 768 x 768:
-// 284 / 264;  10007 x 304 x 203: 21 / 23.
+// 271 / 208 (the cutting of the gradients serves twice the columns);  16384 x 384 x 384: 28.8 / 31;
+// 10007 x 299 x 203: 22.7 / 24.5.
 struct Tile {
   int f32, bo, bi, tk, places;
   float chunk;
 };
 constexpr Tile kTiles[] = {
     {0, 256, 256, 64, 256, 2.19f}, {0, 256, 128, 64, 256, 1.175f}, {0, 128, 128, 64, 256, 0.8f},
-    {1, 128, 128, 64, 256, 1.85f}, {1, 128, 128, 32, 512, 1.75f},
+    {1, 128, 128, 64, 256, 1.76f}, {1, 128, 256, 32, 256, 1.31f},
 };
 struct Plan {
   int tile, bo, bi, S;
@@ -620,6 +618,6 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
     case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, fast, st);
     case 2: return launch<bf16, 128, 128, 2, 4, 64>(a, fast, st);
     case 3: return launch<float, 128, 128, 2, 4, 64>(a, fast, st);
-    default: return launch<float, 128, 128, 2, 2, 32>(a, fast, st);
+    default: return launch<float, 128, 256, 2, 4, 32>(a, fast, st);
   }
 }
