@@ -105,22 +105,22 @@ __device__ __forceinline__ void lds16(lds_byte* p, uint4 a) {
   *(__attribute__((address_space(3))) u32x4*)p = v;
 }
 
-// Byte offset of (row, 16-B column) in an image of h.  A thread writes two neighbouring columns, 2 x
-// and 2 x + 1, one after the other: the even columns are stored in front of the odd ones, so that
-// eight lanes write 128 B of different banks.  The four rows x four columns that a transposing
-// read takes at a time lie in 16 different places of 256 B, by the exclusive or with the row.
-__device__ __forceinline__ int xoff16(int row, int col) {
-  return 256 * row + 16 * (((col >> 1) | ((col & 1) << 3)) ^ ((row & 3) << 1));
-}
+// LDS images of 128 columns of bf16, a row a token.  A transposing read takes four rows x 64 B at a
+// time: the row pitches are chosen so that these lie in different banks (of 64 x 4 B) without an
+// exclusive or in the address, whose steps -- columns, rows, parts -- are then immediate offsets of one
+// register.  gY: 256 + 64 B.  h: a thread writes two neighbouring 16-B columns, 2 x and 2 x + 1, one
+// after the other; the even columns are stored in front of the odd ones, so that eight lanes write
+// 128 B of different banks, and the pitch is 256 + 32 B.
+constexpr int kPitchG = 320, kPitchX = 288;
 
 // acc += h^T gY over the wave's TO x TI tiles of 32 x 32, chunk by chunk
 template <typename T, int BO, int BI, int WO, int WI, int TK, bool FAST>
 __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;   // parts of a gradient
   constexpr int NT = 64 * WO * WI, TO = BO / WO / 32, TI = BI / WI / 32;
-  constexpr int kImg = TK * 256;                              // bytes of an image: TK tokens x 128 bf16
+  constexpr int kImgG = TK * kPitchG, kImgX = TK * kPitchX;   // bytes of an image
   constexpr int NHO = BO / 128, NHI = BI / 128;               // images of a part of gY, of h
-  constexpr int kStage = (NP * NHO + NHI) * kImg;
+  constexpr int kStage = NP * NHO * kImgG + NHI * kImgX;
   constexpr int GC = BO / 8, XC = BI / 16;                    // pieces of a token: 8 gradients, 16 of q
   constexpr int GP = TK * GC / NT, XP = TK * XC / NT;         // pieces of a thread
   constexpr int KS = TK / 16;                                 // MFMA steps of a chunk
@@ -189,32 +189,19 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
     left -= TK;
     size_up();
   };
-  // LDS addresses, all of the current stage: the pieces' places (a piece's rows are 16 apart or a
-  // multiple: the swizzle is the same) and the operands' (tr_frag: rows k.., 4 rows on, columns)
+  // LDS addresses, all of the current stage: this thread's pieces and its wave's operands.  An operand
+  // of 16 tokens x 32 columns is two transposing reads: rows 8 hh + (l & 15) / 4 and four rows on,
+  // columns (l & 16) + 4 (l & 3)..
   typedef __attribute__((address_space(3))) bf16x4v_t lds_v4;
-  static_assert((NT / GC) % 16 == 0 && (NT / XC) % 16 == 0, "a thread's pieces have one swizzle");
   lds_byte* const base = (lds_byte*)smem;
-  lds_byte* at_g = base + (gc >> 4) * kImg + woff(gr, gc & 15);
-  lds_byte* at_x[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) at_x[h] = base + (NP * NHO + (xc >> 3)) * kImg + xoff16(xr, 2 * (xc & 7) + h);
-  lds_byte *at_b[TO][2], *at_a[TI][2];
-  {
-    const int row = 8 * hh + ((l & 15) >> 2), col = (l & 16) + 4 * (l & 3);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int to = 0; to < TO; ++to) {
-        const int c = ((wo + 32 * to) & 127) + col;
-        at_b[to][h] = base + ((wo + 32 * to) >> 7) * kImg + woff(row + 4 * h, c >> 3) + (c & 7) * 2;
-      }
-#pragma unroll
-      for (int ti = 0; ti < TI; ++ti) {
-        const int c = ((wi + 32 * ti) & 127) + col;
-        at_a[ti][h] = base + (NP * NHO + ((wi + 32 * ti) >> 7)) * kImg + xoff16(row + 4 * h, c >> 3) + (c & 7) * 2;
-      }
-    }
-  }
+  lds_byte* at_g = base + (gc >> 4) * kImgG + gr * kPitchG + (gc & 15) * 16;
+  lds_byte* at_x = base + NP * NHO * kImgG + (xc >> 3) * kImgX + xr * kPitchX + (xc & 7) * 16;
+  const int orow = 8 * hh + ((l & 15) >> 2);
+  lds_byte* at_b = base + (wo >> 7) * kImgG + orow * kPitchG + ((wo & 127) + (l & 16) + 4 * (l & 3)) * 2;
+  lds_byte* at_a = base + NP * NHO * kImgG + (wi >> 7) * kImgX + orow * kPitchX + (wi & 127) + (l & 16) +
+                   ((l & 2) >> 1) * 128 + (l & 1) * 8;
+  static_assert(BO / WO <= 128 && BI / WI <= 128 && 128 % (BO / WO) == 0 && 128 % (BI / WI) == 0,
+                "a wave's operands lie in one image");
   // db: this thread's columns of gY, summed as they pass.  The workgroups of an output block share a
   // split's chunks, this one's are [b0, b1); the first workgroup has them all where there is no
   // second kernel to add them up, and on the largest tile, which has no registers for a third loop
@@ -230,7 +217,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   for (int i = 0; i < 8; ++i) bsum[i] = 0.f;
   auto put_g = [&](int p, auto bias_tag) {
     constexpr bool BIAS = decltype(bias_tag)::value;
-    lds_byte* to = at_g + p * (NT / GC) * 256;
+    lds_byte* to = at_g + p * (NT / GC) * kPitchG;
     float v[8];
     if constexpr (NP == 3 || BIAS) g[p].unpack(v);
     if constexpr (BIAS) {
@@ -241,8 +228,8 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
       uint4 hi, mid, lo;
       split3(v, hi, mid, lo);
       lds16(to, hi);
-      lds16(to + NHO * kImg, mid);
-      lds16(to + 2 * NHO * kImg, lo);
+      lds16(to + NHO * kImgG, mid);
+      lds16(to + 2 * NHO * kImgG, lo);
     } else {
       lds16(to, g[p].a);
     }
@@ -256,13 +243,12 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
 #pragma unroll
       for (int i = 0; i < 4; ++i)                // exact in bf16: the upper halves
         o[i] = __builtin_amdgcn_perm(__float_as_uint(v[2 * i + 1]), __float_as_uint(v[2 * i]), 0x07060302u);
-      lds16(at_x[h] + p * (NT / XC) * 256, make_uint4(o[0], o[1], o[2], o[3]));
+      lds16(at_x + p * (NT / XC) * kPitchX + h * 128, make_uint4(o[0], o[1], o[2], o[3]));
     }
   };
   auto to_stage = [&](int step) {                // where the pieces go, `step` stages on
     at_g += step * kStage;
-    at_x[0] += step * kStage;
-    at_x[1] += step * kStage;
+    at_x += step * kStage;
   };
 
   f32x16_t acc[TO][TI];
@@ -298,27 +284,23 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
     lds_barrier();
     // operands of a step of 16 tokens, read one step ahead
     bf16x8_t xa[2][TI], gb[2][TO][NP];
-    auto operand = [&](lds_byte* const (&p)[2], int offset) {
-      const bf16x4v_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p[0] + offset));
-      const bf16x4v_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p[1] + offset));
+    auto operand = [&](lds_byte* p, int pitch) {
+      const bf16x4v_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p);
+      const bf16x4v_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p + 4 * pitch));
       return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
     auto read = [&](int k, int f) {
 #pragma unroll
-      for (int ti = 0; ti < TI; ++ti) xa[f][ti] = operand(at_a[ti], 16 * 256 * k);
+      for (int ti = 0; ti < TI; ++ti) xa[f][ti] = operand(at_a + 16 * kPitchX * k + 32 * ti, kPitchX);
 #pragma unroll
       for (int to = 0; to < TO; ++to)
 #pragma unroll
-        for (int p = 0; p < NP; ++p) gb[f][to][p] = operand(at_b[to], p * NHO * kImg + 16 * 256 * k);
+        for (int p = 0; p < NP; ++p)
+          gb[f][to][p] = operand(at_b + p * NHO * kImgG + 16 * kPitchG * k + 64 * to, kPitchG);
     };
     auto next_stage = [&](int step) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int to = 0; to < TO; ++to) at_b[to][h] += step * kStage;
-#pragma unroll
-        for (int ti = 0; ti < TI; ++ti) at_a[ti][h] += step * kStage;
-      }
+      at_b += step * kStage;
+      at_a += step * kStage;
     };
     static_assert(KS % 2 == 0, "the operands' two sets alternate over chunks");
     int flip = 1;                                // from the stage that is read to the other one
@@ -550,7 +532,7 @@ long long workspace_bytes(const Plan& p, int N, int K) {
 template <typename T, int BO, int BI, int WO, int WI, int TK>
 int launch(const Wgrad8& a, bool fast, hipStream_t st) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;
-  constexpr int kLds = 2 * (NP * BO / 128 + BI / 128) * TK * 256;
+  constexpr int kLds = 2 * TK * (NP * (BO / 128) * kPitchG + (BI / 128) * kPitchX);
   const auto kernel = fast ? act8_wgrad_kernel<T, BO, BI, WO, WI, TK, true>
                            : act8_wgrad_kernel<T, BO, BI, WO, WI, TK, false>;
   if (kLds > 64 * 1024)                          // above the default limit of a launch
