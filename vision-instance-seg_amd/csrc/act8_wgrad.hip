@@ -2,8 +2,8 @@
 //     dW[o, i] = sum_t gY[t, o] h[t, i],   db[o] = sum_t gY[t, o],   h[t, i] = q[t, i] 2^e[t, i / 32]
 //
 // The reduction runs over tokens, the strided dimension of both operands: 64-token chunks are
-// staged in LDS in their natural [token][feature] order (images of 128 columns, lds_dma.h) and
-// read as MFMA operands with the transposing LDS read.  The checkpoint is widened to bf16 on its
+// staged in LDS in their natural [token][feature] order (images of 128 columns, padded row
+// pitches: kPitchG, kPitchX) and read as MFMA operands with the transposing LDS read.  The checkpoint is widened to bf16 on its
 // way into LDS, once a workgroup, exactly (act8.h).  f32 gradients are cut into three bf16 parts
 // by truncation, gY = hi + mid + lo: 8 bits of significand each, so the sum is exact, and three
 // matrix products give what an f32 product of exact terms would; a non-finite value is its hi
@@ -18,15 +18,15 @@
 // What bounds it.  Vector arithmetic costs MFMA time almost in full (64 idle instructions more a
 // chunk: 10 to 16 % more time), so the widening of the checkpoint, 2.5 instructions an element, is
 // what an uncompressed operand would save; at large sizes the clock falls to ~1.6 GHz with the matrix
-// units busy 68 % of the cycles.  Measured: 147456 tokens x 1024 x 2048 bf16 540-595 us (1040-1145
-// TF/s; the library's 8192^3 product 1475, its product at these sizes and layouts 570);  16384 x
-// 1536 x 384 35.8 us, of it 7.7 for the sum of 14 splits (33 MB of partials; the products alone are
-// 13 us at the library's rate);  262144 x 96 x 384 47.5;  400 x 256 x 256 9.5 (seven chunks in a
-// row: latency);  f32 65536 x 768 x 768 208
-// (372 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 17.5 + 4.
+// units busy 68 % of the cycles.  Measured on several cards (they differ by up to 15 %):  147456
+// tokens x 1024 x 2048 bf16 540-595 us (1040-1145 TF/s; the library's 8192^3 product 1475, its
+// product at these sizes and layouts 570);  16384 x 1536 x 384 35-37 us, of it 7.7 for the sum of 14
+// splits (33 MB of partials; the products alone are 13 us at the library's rate);  262144 x 96 x 384
+// 44-47;  400 x 256 x 256 9-10 (seven chunks in a row: latency);  f32 65536 x 768 x 768 210-250
+// (310-370 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 18.5 + 4.
 // Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
-// chunks in flight in registers (the loads are not what it waits for), a 128 x 128 tile a wave (four
-// waves of 256 x 256: spills).
+// chunks in flight in registers (the loads are not what it waits for; the first two asked for at once:
+// no change), a 128 x 128 tile a wave (four waves of 256 x 256: spills).
 #include <type_traits>
 
 #include "act8.h"
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a)
 // quarter, ... of them).  Measured as tile 0 / 1 / 2, us:  147456 tokens x 1024 x 2048: 635 / 677 /
 // 790;  65536 x 768 x 192: 48 / 42 / 52;  16384 x 1536 x 384: 45 / 37 / 41;  262144 x 96 x 384: 79 /
 // 67 / 52;  400 x 256 x 256: 20 / 13 / 9.5 (12 in two splits).  f32, tile 3 / 4: 65536 x 768 x 768:
-// 271 / 208 (the cutting of the gradients serves twice the columns);  16384 x 384 x 384: 28.8 / 31;
+// 271 / 210-250 (the cutting of the gradients serves twice the columns);  16384 x 384 x 384: 28.8 / 31;
 // 10007 x 299 x 203: 22.7 / 24.5.
 struct Tile {
   int f32, bo, bi, tk, places;
@@ -592,9 +592,9 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
   a.part = (float*)workspace;
   a.pbias = a.part + (size_t)a.S * a.tiles * (plan.bo * plan.bi);
   hipStream_t st = (hipStream_t)stream;
-  // buffer loads: aligned rows, and a chunk of rows within their 32-bit offsets
+  // buffer loads take dwords: rows that begin on one, and a chunk of rows within their 32-bit offsets
   const long long esz = dtype == VS_F32 ? 4 : 2;
-  const bool fast = ((uintptr_t)gy & 15) == 0 && ld_gy * esz % 16 == 0 && 64 * (ld_gy + N) * esz < (1ll << 31);
+  const bool fast = ((uintptr_t)gy & 3) == 0 && ld_gy * esz % 4 == 0 && 64 * (ld_gy + N) * esz < (1ll << 31);
   switch (plan.tile) {
     case 0: return launch<bf16, 256, 256, 2, 4, 64>(a, fast, st);
     case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, fast, st);
