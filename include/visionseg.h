@@ -302,7 +302,7 @@ VS_API int vs_act8_gelu_backward(int dtype, const void* gy, const void* q, const
 /* LayerNorm over the features (<= 8192) of x, or -- r and s not NULL -- of s = x + r, rounded to
  * dtype and written: y = (x - mean) * rstd * w + b, mean / rstd f32 [rows], and the checkpoint
  * of the normalised tensor (q and scale NULL: none).  y_rows int32 [rows] (may be NULL): the
- * row of y [y_count, features] that row i goes to (outside it: nowhere). */
+ * row of y [y_count, features] that row i goes to (outside it: nowhere; no two rows to one). */
 VS_API int vs_act8_layer_norm_forward(int dtype, const void* x, const void* r, const void* w, const void* b, void* s,
                                       void* y, void* q, void* scale, float* mean, float* rstd, long long rows,
                                       int features, float eps, const int* y_rows, long long y_count, void* stream);

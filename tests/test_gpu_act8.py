@@ -719,3 +719,37 @@ def test_rows_beyond_32_bits():
     dw = ops.act8_wgrad(gy, q, s, C, F32)
     rw, _, tw, _ = ref.wgrad(gs, rq, rs, C, F32)
     ref.within(dw, rw, tw, "dw")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,K,N,pitch,first", [
+    (1, 40, 9, 9, 1), (130, 40, 9, 9, 1), (130, 40, 9, 11, 2), (1000, 300, 517, 517, 0), (1000, 300, 517, 519, 1),
+    (1000, 300, 518, 519, 3), (6000, 515, 515, 515, 0), (6000, 515, 514, 514, 1), (9000, 1030, 1031, 1031, 1)])
+def test_wgrad_row_starts(T, K, N, pitch, first, dtype):
+    """Rows that begin anywhere; the gradient's last value is its storage's last, and what lies in
+    front of a row and behind it is NaN."""
+    ops = _ops()
+    q, s = ops.act8_pack(_act(T, K, dtype, 5))
+    flat = torch.full((first + (T - 1) * pitch + N,), float("nan"), device=DEV, dtype=dtype)
+    gy = flat.as_strided((T, N), (pitch, 1), first)
+    gy.copy_(_grad(T, N, dtype, 6))
+    dw, db = ops.act8_wgrad(gy, q, s, K, F32, bias=True)
+    rw, rb, tw, tb = ref.wgrad(gy.contiguous(), q, s, K, F32)
+    ref.within(dw, rw, tw, "dw")
+    ref.within(db, rb, tb, "db")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N", [40, 257])
+def test_wgrad_rows_far_apart(N, dtype):
+    """64 rows that span more than 2^31 bytes: addressed row by row."""
+    ops = _ops()
+    T, K, pitch = 70, 100, 1 << 24
+    q, s = ops.act8_pack(_act(T, K, dtype, 7))
+    flat = torch.empty((T - 1) * pitch + N, device=DEV, dtype=dtype)
+    gy = flat.as_strided((T, N), (pitch, 1))
+    gy.copy_(_grad(T, N, dtype, 8))
+    dw, db = ops.act8_wgrad(gy, q, s, K, F32, bias=True)
+    rw, rb, tw, tb = ref.wgrad(gy.contiguous(), q, s, K, F32)
+    ref.within(dw, rw, tw, "dw")
+    ref.within(db, rb, tb, "db")

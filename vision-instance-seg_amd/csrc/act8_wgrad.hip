@@ -27,6 +27,7 @@
 // Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
 // chunks in flight in registers (the loads are not what it waits for; the first two asked for at once:
 // no change), a 128 x 128 tile a wave (four waves of 256 x 256: spills).
+#include <climits>
 #include <type_traits>
 
 #include "act8.h"
@@ -113,8 +114,15 @@ __device__ __forceinline__ void lds16(lds_byte* p, uint4 a) {
 // 128 B of different banks, and the pitch is 256 + 32 B.
 constexpr int kPitchG = 320, kPitchX = 288;
 
+// How gY is loaded.  Rows: by address, each row and chunk checked against its end (any stride; the
+// branches drain the loads in flight).  Dwords: buffer loads, of rows that begin on a dword.  Halves:
+// buffer loads of the 20 B around a chunk of bf16, from the dword that its first value lies in, and a
+// shift by 0 or 16 bits on the way into LDS (40001 x 1030 x 1030 bf16, row pitch 1030 / 1031 values:
+// 130 / 142 us; by rows 238).
+enum Feed { kRows, kDwords, kHalves };
+
 // acc += h^T gY over the wave's TO x TI tiles of 32 x 32, chunk by chunk
-template <typename T, int BO, int BI, int WO, int WI, int TK, bool FAST>
+template <typename T, int BO, int BI, int WO, int WI, int TK, int FEED>
 __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;   // parts of a gradient
   constexpr int NT = 64 * WO * WI, TO = BO / WO / 32, TI = BI / WI / 32;
@@ -138,6 +146,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   const int gr = threadIdx.x / GC, gc = threadIdx.x % GC, xr = threadIdx.x / XC, xc = threadIdx.x % XC;
   const int gcol = ob * BO + gc * 8, xcol = ib * BI + xc * 16;
   Chunk<T> g[GP];
+  uint32_t tail[FEED == kHalves ? GP : 1];       // the dword behind a chunk
   uint4 xq[XP];
   uint32_t xs[XP];
   // The next chunk to fetch: the three tensors from its first row on, and the rows left.  A buffer
@@ -150,24 +159,34 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   const unsigned char* sbase = a.scale + cb_rows * (a.P >> 5);
   const long long end = (long long)ce * TK;      // (behind the split's last chunk too: zeros)
   int left = (int)((end < a.T ? end : a.T) - cb_rows);
-  const int gld = (int)(a.ldg * (long long)sizeof(T)), sld = a.P >> 5;        // (gld: the FAST path's)
-  const int goff = gr * gld + gcol * (int)sizeof(T), xoff = xr * a.P + xcol, soff = xr * sld + (xcol >> 5);
-  const int gap = gld - ((a.N * (int)sizeof(T) + 3) & ~3);                    // behind a row's last dword
+  const int gld = (int)(a.ldg * (long long)sizeof(T)), sld = a.P >> 5;        // (gld: the buffer loads')
+  // kHalves: where gbase lies in its dword -- in every chunk, TK rows on, the same -- and a thread's
+  // chunks in theirs: its rows are an even number apart
+  static_assert(FEED != kHalves || (sizeof(T) == 2 && (NT / GC) % 2 == 0 && TK % 2 == 0), "one shift a thread");
+  const int odd = FEED == kHalves ? (int)(reinterpret_cast<uintptr_t>(gbase) & 2) : 0;
+  gbase -= odd;
+  const int gbyte = odd + gr * gld + gcol * (int)sizeof(T), gshift = (gbyte & 2) * 8;
+  const int goff = FEED == kHalves ? gbyte & ~3 : gbyte;
+  const int xoff = xr * a.P + xcol, soff = xr * sld + (xcol >> 5);
+  const int gap = gld - odd - a.N * (int)sizeof(T) - 3;      // (rows gld - gap) & ~3: to the last row's last dword
   // the chunk's bytes (readfirstlane: buffer descriptors live in scalar registers)
   int gsize, qsize, ssize;
   auto size_up = [&]() {
     const int rows = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : left < TK ? left : TK);
-    const int g0 = rows * gld - gap;
-    gsize = __builtin_amdgcn_readfirstlane(g0 < 0 ? 0 : g0);
+    gsize = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows * gld - gap) & ~3 : 0);
     qsize = rows * a.P;
     ssize = rows * sld;
   };
   size_up();
   auto fetch_g = [&](int p) {
-    if constexpr (FAST) {
+    if constexpr (FEED != kRows) {
       const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)gbase, 0, gsize, 0x00020000);
-      g[p].a = buffer16(rs, goff + p * (NT / GC) * gld);
-      if constexpr (NP == 3) g[p].b = buffer16(rs, goff + p * (NT / GC) * gld + 16);
+      int at = goff + p * (NT / GC) * gld;
+      // (the row behind the last one can begin in the last one's last dword)
+      if constexpr (FEED == kHalves) at = p * (NT / GC) < left - gr ? at : INT_MIN;
+      g[p].a = buffer16(rs, at);
+      if constexpr (FEED == kHalves) tail[p] = __builtin_amdgcn_raw_buffer_load_b32(rs, at + 16, 0, 0);
+      if constexpr (NP == 3) g[p].b = buffer16(rs, at + 16);
     } else {
       const int row = p * (NT / GC) + gr;
       if (row < left)
@@ -218,6 +237,11 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   auto put_g = [&](int p, auto bias_tag) {
     constexpr bool BIAS = decltype(bias_tag)::value;
     lds_byte* to = at_g + p * (NT / GC) * kPitchG;
+    if constexpr (FEED == kHalves) {
+      const uint4 d = g[p].a;
+      g[p].a = make_uint4(__builtin_amdgcn_alignbit(d.y, d.x, gshift), __builtin_amdgcn_alignbit(d.z, d.y, gshift),
+                          __builtin_amdgcn_alignbit(d.w, d.z, gshift), __builtin_amdgcn_alignbit(tail[p], d.w, gshift));
+    }
     float v[8];
     if constexpr (NP == 3 || BIAS) g[p].unpack(v);
     if constexpr (BIAS) {
@@ -530,11 +554,13 @@ long long workspace_bytes(const Plan& p, int N, int K) {
 }
 
 template <typename T, int BO, int BI, int WO, int WI, int TK>
-int launch(const Wgrad8& a, bool fast, hipStream_t st) {
+int launch(const Wgrad8& a, Feed feed, hipStream_t st) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;
   constexpr int kLds = 2 * TK * (NP * (BO / 128) * kPitchG + (BI / 128) * kPitchX);
-  const auto kernel = fast ? act8_wgrad_kernel<T, BO, BI, WO, WI, TK, true>
-                           : act8_wgrad_kernel<T, BO, BI, WO, WI, TK, false>;
+  auto kernel = feed == kRows ? act8_wgrad_kernel<T, BO, BI, WO, WI, TK, kRows>
+                              : act8_wgrad_kernel<T, BO, BI, WO, WI, TK, kDwords>;
+  if constexpr (NP == 1)
+    if (feed == kHalves) kernel = act8_wgrad_kernel<T, BO, BI, WO, WI, TK, kHalves>;
   if (kLds > 64 * 1024)                          // above the default limit of a launch
     VS_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.S * a.tiles)), dim3(64 * WO * WI), kLds, st, a);
@@ -570,6 +596,7 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
   VS_CHECK((K == 0 || dw) && (tokens == 0 || (gy && (K == 0 || (q && scale)))), "null pointer");
   VS_CHECK(((uintptr_t)q & 15) == 0, "q must be 16-B aligned");
   VS_CHECK(K > 0, "K > 0");
+  VS_CHECK(((uintptr_t)gy & (dtype == VS_F32 ? 3 : 1)) == 0, "gy must be aligned to its elements");
   Wgrad8 a;
   a.gy = gy;
   a.q = (const unsigned char*)q;
@@ -592,14 +619,16 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
   a.part = (float*)workspace;
   a.pbias = a.part + (size_t)a.S * a.tiles * (plan.bo * plan.bi);
   hipStream_t st = (hipStream_t)stream;
-  // buffer loads take dwords: rows that begin on one, and a chunk of rows within their 32-bit offsets
+  // buffer loads: a chunk of rows within their 32-bit offsets
   const long long esz = dtype == VS_F32 ? 4 : 2;
-  const bool fast = ((uintptr_t)gy & 3) == 0 && ld_gy * esz % 4 == 0 && 64 * (ld_gy + N) * esz < (1ll << 31);
+  const Feed feed = 64 * (ld_gy + N) * esz >= (1ll << 31)                     ? kRows
+                    : (((uintptr_t)gy & 3) == 0 && ld_gy * esz % 4 == 0) ? kDwords
+                                                                         : kHalves;
   switch (plan.tile) {
-    case 0: return launch<bf16, 256, 256, 2, 4, 64>(a, fast, st);
-    case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, fast, st);
-    case 2: return launch<bf16, 128, 128, 2, 4, 64>(a, fast, st);
-    case 3: return launch<float, 128, 128, 2, 4, 64>(a, fast, st);
-    default: return launch<float, 128, 256, 2, 4, 32>(a, fast, st);
+    case 0: return launch<bf16, 256, 256, 2, 4, 64>(a, feed, st);
+    case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, feed, st);
+    case 2: return launch<bf16, 128, 128, 2, 4, 64>(a, feed, st);
+    case 3: return launch<float, 128, 128, 2, 4, 64>(a, feed, st);
+    default: return launch<float, 128, 256, 2, 4, 32>(a, feed, st);
   }
 }

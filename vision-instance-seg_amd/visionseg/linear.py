@@ -1074,7 +1074,8 @@ def _act8_ready(x, *params) -> bool:
 
 def linear_act8(x, w, b=None):
     """F.linear(x, w, b) whose weight gradient reads x's 8-bit checkpoint (ops.act8_pack) instead
-    of x.  Plain F.linear where no weight gradient is wanted: nothing of x is kept then."""
+    of x.  Plain F.linear where no weight gradient is wanted (nothing of x is kept then), on the
+    CPU and for other dtypes than f32 / bf16."""
     if torch.is_autocast_enabled() and x.is_cuda:
         dt = torch.get_autocast_dtype("cuda")
         with torch.autocast("cuda", enabled=False):
@@ -1086,7 +1087,8 @@ def linear_act8(x, w, b=None):
 
 def mlp_act8(x, w1, b1, w2, b2):
     """fc2(gelu(fc1(x))) (exact GELU; w1 [hidden, C], w2 [C', hidden]) that keeps 8-bit
-    checkpoints of x and of the pre-activation and nothing else (see _MlpAct8Fn)."""
+    checkpoints of x and of the pre-activation and nothing else (see _MlpAct8Fn); the plain
+    composition where linear_act8 is plain F.linear."""
     if torch.is_autocast_enabled() and x.is_cuda:
         dt = torch.get_autocast_dtype("cuda")
         with torch.autocast("cuda", enabled=False):

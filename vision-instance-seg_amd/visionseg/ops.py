@@ -1548,8 +1548,8 @@ def activation(x, kind: str, gelu_sink=None):
 # magnitude is at most 127 steps, so a value is off by at most 1 / 127 of its block's largest and
 # is exact in bf16.  `q` int8 [..., P] (P = the features rounded up to 32, zeros behind them),
 # `scale` uint8 [..., P / 32] = e + 127; a block with an infinity or a NaN (or a magnitude
-# above 127 * 2^121) is kept as NaN (scale 255).  The forward results are not touched: only the backward formulas are taken at the
-# checkpointed values.
+# above 127 * 2^121) is kept as NaN (scale 255).  The forward results are not touched: only the
+# backward formulas are taken at the checkpointed values.
 _ACT8 = None
 
 
