@@ -1087,8 +1087,8 @@ def linear_act8(x, w, b=None):
 
 def mlp_act8(x, w1, b1, w2, b2):
     """fc2(gelu(fc1(x))) (exact GELU; w1 [hidden, C], w2 [C', hidden]) that keeps 8-bit
-    checkpoints of x and of the pre-activation and nothing else (see _MlpAct8Fn); the plain
-    composition where linear_act8 is plain F.linear."""
+    checkpoints of x and of the pre-activation and nothing else (see _MlpAct8Fn).  The plain
+    composition where no gradient is wanted, on the CPU and for other dtypes than f32 / bf16."""
     if torch.is_autocast_enabled() and x.is_cuda:
         dt = torch.get_autocast_dtype("cuda")
         with torch.autocast("cuda", enabled=False):
