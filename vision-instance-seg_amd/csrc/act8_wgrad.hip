@@ -341,11 +341,13 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
             // the steps before, MFMA by MFMA with a share of the operand reads and of the pieces'
             // arithmetic behind each (alone on the chip 1257 ns a chunk against 1374 as the compiler
             // has it; the smaller tiles lose by it).  2 and 4 vector instructions: 530 us at 147456 x
-            // 1024 x 2048; 3 and 5: 537, 4 and 6: 547, one LDS read an MFMA: 573
+            // 1024 x 2048; 3 and 5: 537, 4 and 6: 547, one LDS read an MFMA: 573.  kHalves with db:
+            // 6 (4: the loop spills, 1282 us at 147456 x 1025 x 2047 against 733)
+            constexpr int kVector = !decltype(bias_tag)::value ? 2 : FEED == kHalves ? 6 : 4;
 #pragma unroll
             for (int i = 0; i < (KS - 1) * TO * TI; ++i) {
               __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);      // MFMA
-              __builtin_amdgcn_sched_group_barrier(0x2, decltype(bias_tag)::value ? 4 : 2, 0);      // vector arithmetic
+              __builtin_amdgcn_sched_group_barrier(0x2, kVector, 0);// vector arithmetic
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);    // LDS reads
             }
           }
