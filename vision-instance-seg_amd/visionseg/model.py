@@ -70,8 +70,8 @@ class M2FConfig:
     # backward in bf16)
     linear_fp8: bool = False
     # the Swin blocks keep what their norms, qkv projections and MLPs need for the backward pass
-    # as 8-bit activation checkpoints (ops.act8_pack): same forward results, about half the
-    # activation memory; not together with linear_fp8
+    # as 8-bit activation checkpoints (ops.act8_pack): the same forward pass, to rounding, about
+    # half the activation memory; not together with linear_fp8
     act8: bool = False
 
     @staticmethod
