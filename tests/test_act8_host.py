@@ -113,3 +113,10 @@ def test_config_switch():
     assert not any(blk.act8 or blk.mlp.act8 for st in SwinBackbone(M2FConfig()).stages for blk in st.blocks)
     with pytest.raises(ValueError, match="act8"):
         SwinBackbone(M2FConfig.preset("swin_t", act8=True, linear_fp8=True))
+
+
+def test_wgrad_refuses_gradients_off_their_alignment():
+    lib = L.lib()
+    for dtype, address in ((0, 18), (1, 17)):                 # f32 on 2 B, bf16 on 1 B
+        rc = lib.vs_act8_wgrad(dtype, 1, ctypes.c_void_p(address), 8, P16, P16, P16, P16, P16, 4, 8, 8, None)
+        assert rc == -1 and b"aligned to its elements" in lib.vs_last_error()
