@@ -753,3 +753,19 @@ def test_wgrad_rows_far_apart(N, dtype):
     rw, rb, tw, tb = ref.wgrad(gy.contiguous(), q, s, K, F32)
     ref.within(dw, rw, tw, "dw")
     ref.within(db, rb, tb, "db")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,K,N", [(100000, 20, 18), (200000, 96, 95), (200000, 96, 96), (16384, 384, 1536),
+                                   (40001, 1030, 1030), (40001, 1029, 1031)])
+def test_wgrad_tiles(T, K, N, dtype):
+    """Sizes from the smallest output tile with hundreds of splits to the largest one."""
+    ops = _ops()
+    x, gy = _act(T, K, dtype, 9), _grad(T, N, dtype, 10)
+    q, s = ops.act8_pack(x)
+    del x
+    dw, db = ops.act8_wgrad(gy, q, s, K, F32, bias=True)
+    rw, rb, tw, tb = ref.wgrad(gy, q, s, K, F32)
+    ref.within(dw, rw, tw, "dw")
+    ref.within(db, rb, tb, "db")
+    assert torch.equal(ops.act8_wgrad(gy, q, s, K, F32), dw)

@@ -22,8 +22,8 @@
 // tokens x 1024 x 2048 bf16 540-595 us (1040-1145 TF/s; the library's 8192^3 product 1475, its
 // product at these sizes and layouts 570);  16384 x 1536 x 384 35-37 us, of it 7.7 for the sum of 14
 // splits (33 MB of partials; the products alone are 13 us at the library's rate);  262144 x 96 x 384
-// 44-47;  400 x 256 x 256 9-10 (seven chunks in a row: latency);  f32 65536 x 768 x 768 210-250
-// (310-370 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 18.5 + 4.
+// 44-47;  400 x 256 x 256 7 (seven chunks in a row);  f32 65536 x 768 x 768 210-250
+// (310-370 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 18.
 // Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
 // chunks in flight in registers (the loads are not what it waits for; the first two asked for at once:
 // no change), a 128 x 128 tile a wave (four waves of 256 x 256: spills).
@@ -113,6 +113,7 @@ __device__ __forceinline__ void lds16(lds_byte* p, uint4 a) {
 // after the other; the even columns are stored in front of the odd ones, so that eight lanes write
 // 128 B of different banks, and the pitch is 256 + 32 B.
 constexpr int kPitchG = 320, kPitchX = 288;
+constexpr int images(int columns) { return (columns + 127) / 128; }
 
 // How gY is loaded.  Rows: by address, each row and chunk checked against its end (any stride; the
 // branches drain the loads in flight).  Dwords: buffer loads, of rows that begin on a dword.  Halves:
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(64 * WO * WI) act8_wgrad_kernel(const Wgrad8 a
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;   // parts of a gradient
   constexpr int NT = 64 * WO * WI, TO = BO / WO / 32, TI = BI / WI / 32;
   constexpr int kImgG = TK * kPitchG, kImgX = TK * kPitchX;   // bytes of an image
-  constexpr int NHO = BO / 128, NHI = BI / 128;               // images of a part of gY, of h
+  constexpr int NHO = images(BO), NHI = images(BI);           // images of a part of gY, of h
   constexpr int kStage = NP * NHO * kImgG + NHI * kImgX;
   constexpr int GC = BO / 8, XC = BI / 16;                    // pieces of a token: 8 gradients, 16 of q
   constexpr int GP = TK * GC / NT, XP = TK * XC / NT;         // pieces of a thread
@@ -507,16 +508,20 @@ __global__ void __launch_bounds__(64 * NG) act8_wgrad_sum_kernel(const Wgrad8 a)
 // (us; a place is a workgroup that runs at a time: splits fill the places once, or a half, a
 // quarter, ... of them).  Measured as tile 0 / 1 / 2, us:  147456 tokens x 1024 x 2048: 635 / 677 /
 // 790;  65536 x 768 x 192: 48 / 42 / 52;  16384 x 1536 x 384: 45 / 37 / 41;  262144 x 96 x 384: 79 /
-// 67 / 52;  400 x 256 x 256: 20 / 13 / 9.5 (12 in two splits).  f32, tile 3 / 4: 65536 x 768 x 768:
-// 271 / 210-250 (the cutting of the gradients serves twice the columns);  16384 x 384 x 384: 28.8 / 31;
-// 10007 x 299 x 203: 22.7 / 24.5.
+// 67 / 52.  Tile 2 / 3:  400 x 256 x 256: 8.6 / 7.0 (12 in two splits);  10007 x 203 x 299: 15.5 /
+// 13.7;  262144 x 96 x 96: 22.3 / 26;  262144 x 96 x 384: 44 / 58;  300000 x 20 x 64: 24 / 15.  f32,
+// tile 4 / 5: 65536 x 768 x 768: 271 / 210-250 (the cutting of the gradients serves twice the
+// columns);  16384 x 384 x 384: 28.8 / 31;  4 / 6: 400 x 256 x 256: 9.8 / 8.7;  10007 x 203 x 299: 19.1 /
+// 18.1;  16384 x 384 x 384: 26 / 35;  300000 x 18 x 20: 40 / 23.
 struct Tile {
   int f32, bo, bi, tk, places;
-  float chunk;
+  float chunk, alone;                            // alone: with at most half the places taken
 };
 constexpr Tile kTiles[] = {
-    {0, 256, 256, 64, 256, 2.19f}, {0, 256, 128, 64, 256, 1.175f}, {0, 128, 128, 64, 256, 0.8f},
-    {1, 128, 128, 64, 256, 1.76f}, {1, 128, 256, 32, 256, 1.31f},
+    {0, 256, 256, 64, 256, 2.19f, 2.19f}, {0, 256, 128, 64, 256, 1.175f, 1.175f},
+    {0, 128, 128, 64, 256, 0.8f, 0.8f},   {0, 64, 64, 64, 512, 0.49f, 0.385f},
+    {1, 128, 128, 64, 256, 1.76f, 1.76f}, {1, 128, 256, 32, 256, 1.31f, 1.31f},
+    {1, 64, 64, 64, 256, 0.62f, 0.62f},
 };
 struct Plan {
   int tile, bo, bi, S;
@@ -536,7 +541,7 @@ Plan plan_of(bool f32, long long T, int N, int K) {
     if (S < 1) S = 1;
     for (; S >= 1; S >>= 1) {
       const long long turns = (tiles * S + t.places - 1) / t.places;
-      float cost = (float)(turns * ((nchunk + S - 1) / S)) * t.chunk + 4.f;
+      float cost = (float)(turns * ((nchunk + S - 1) / S)) * (2 * tiles * S <= t.places ? t.alone : t.chunk) + 4.f;
       if (S > 1) cost += 5.f + 0.2e-6f * (float)(4 * S * tiles * t.bo * t.bi);
       if (best.S == 0 || cost < least) {
         best = {c, t.bo, t.bi, (int)S, tiles};
@@ -559,7 +564,7 @@ long long workspace_bytes(const Plan& p, int N, int K) {
 template <typename T, int BO, int BI, int WO, int WI, int TK>
 int launch(const Wgrad8& a, Feed feed, hipStream_t st) {
   constexpr int NP = std::is_same<T, float>::value ? 3 : 1;
-  constexpr int kLds = 2 * TK * (NP * (BO / 128) * kPitchG + (BI / 128) * kPitchX);
+  constexpr int kLds = 2 * TK * (NP * images(BO) * kPitchG + images(BI) * kPitchX);
   auto kernel = feed == kRows ? act8_wgrad_kernel<T, BO, BI, WO, WI, TK, kRows>
                               : act8_wgrad_kernel<T, BO, BI, WO, WI, TK, kDwords>;
   if constexpr (NP == 1)
@@ -569,9 +574,15 @@ int launch(const Wgrad8& a, Feed feed, hipStream_t st) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.S * a.tiles)), dim3(64 * WO * WI), kLds, st, a);
   VS_LAUNCH_CHECK();
   if (a.S > 1) {
-    constexpr int NG = 4;
     const long long groups = (long long)a.tiles * (BO * BI / 256) + (a.db ? (a.N + 15) / 16 : 0);
-    hipLaunchKernelGGL((act8_wgrad_sum_kernel<BO, BI, WO, WI, NG>), dim3((unsigned)groups), dim3(64 * NG), 0, st, a);
+    auto sum = [&](auto slices) {
+      constexpr int NG = decltype(slices)::value;
+      hipLaunchKernelGGL((act8_wgrad_sum_kernel<BO, BI, WO, WI, NG>), dim3((unsigned)groups), dim3(64 * NG), 0, st, a);
+    };
+    if (a.S > 64)                                // us with 4 / 16: 300000 x 20 x 64 in 512 splits 21.0 / 15.2,
+      sum(std::integral_constant<int, 16>{});    // 262144 x 96 x 96 in 256 24.4 / 22.3,
+    else                                         // 4096 x 768 x 768 in 3 21.1 / 24.6
+      sum(std::integral_constant<int, 4>{});
     VS_LAUNCH_CHECK();
   }
   return VS_OK;
@@ -631,7 +642,9 @@ extern "C" int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long
     case 0: return launch<bf16, 256, 256, 2, 4, 64>(a, feed, st);
     case 1: return launch<bf16, 256, 128, 4, 2, 64>(a, feed, st);
     case 2: return launch<bf16, 128, 128, 2, 4, 64>(a, feed, st);
-    case 3: return launch<float, 128, 128, 2, 4, 64>(a, feed, st);
-    default: return launch<float, 128, 256, 2, 4, 32>(a, feed, st);
+    case 3: return launch<bf16, 64, 64, 2, 2, 64>(a, feed, st);
+    case 4: return launch<float, 128, 128, 2, 4, 64>(a, feed, st);
+    case 5: return launch<float, 128, 256, 2, 4, 32>(a, feed, st);
+    default: return launch<float, 64, 64, 2, 2, 64>(a, feed, st);
   }
 }
