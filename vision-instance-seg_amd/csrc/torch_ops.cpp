@@ -662,9 +662,10 @@ std::tuple<at::Tensor, at::Tensor> act8_wgrad(const at::Tensor& grad_y, const at
   at::Tensor dw = at::empty({N, features}, g.options().dtype(dtype));
   at::Tensor db = at::empty({bias ? N : 0}, g.options().dtype(dtype));
   const int n = as_int(N, "outputs"), k = (int)features;
-  at::Tensor ws = at::empty({vs_act8_wgrad_workspace_bytes(dcode(g), T, n, k)}, g.options().dtype(at::kByte));
+  const int64_t bytes = vs_act8_wgrad_workspace_bytes(dcode(g), T, n, k);
+  at::Tensor ws = bytes ? at::empty({bytes}, g.options().dtype(at::kByte)) : at::Tensor();
   vs_ok(vs_act8_wgrad(dcode(g), dcode(dw), g.data_ptr(), g.stride(0), qc.data_ptr(), sc.data_ptr(), dw.data_ptr(),
-                      bias ? db.data_ptr() : nullptr, ws.data_ptr(), T, n, k, cur_stream(g)),
+                      bias ? db.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, T, n, k, cur_stream(g)),
         "act8_wgrad");
   return {dw, db};
 }
