@@ -7,9 +7,8 @@ shorter where 32 does not divide C).  A block with the largest magnitude a keeps
     e = the smallest integer >= -126 with a <= 127 * 2^e,   q = round_half_even(x * 2^-e)
 
 as `q` int8 [..., P] (P = C rounded up to a multiple of 32, zeros behind C) and `scale` uint8
-[..., P / 32] = e + 127; it stands for q * 2^e, which bfloat16 holds exactly.  A block with a
-magnitude above 127 * 2^121 (the last step before 2^128), an infinity or a NaN has scale 255 and
-q 0 and stands for NaN.
+[..., P / 32] = e + 127; it stands for q * 2^e, which bfloat16 holds exactly.  A block with an
+infinity or a NaN has scale 255 and q 0 and stands for NaN.
 
 Kinds of cases, one per operator:
     pack    write a checkpoint of x and read it back (its values, in x's type)
@@ -154,7 +153,7 @@ def _plain_pack(x):
     pad = -cols % BLOCK
     v = torch.nn.functional.pad(x.float(), (0, pad)).view(rows, -1, BLOCK)
     amax = v.abs().amax(-1)
-    bad = ~(amax <= 127 * 2.0 ** 121)
+    bad = ~torch.isfinite(amax)
     # the exponent from the bits of a float32: a <= 127 * 2^e where its mantissa is <= 1.984375
     bits = amax.view(torch.int32)
     scale = torch.clamp(((bits + 0x1FFFF) >> 23) - 6, min=1)
