@@ -1061,7 +1061,7 @@ class _MlpAct8Fn(torch.autograd.Function):
         elif ctx.has_bias[0] and need[2]:
             gb1 = gh.sum(0, dtype=torch.float32).to(w1.dtype)
         gx = _dgrad_gemm(gh, w1, ctx.wt[0]).view(ctx.shape) if need[0] else None
-        ctx.wt = None
+        ctx.wt = (None, None)                    # (a second backward transposes for itself)
         return gx, gw1, gb1, gw2, gb2
 
 
