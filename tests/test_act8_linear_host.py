@@ -38,3 +38,22 @@ def test_a_second_backward_over_a_retained_graph(plain_kernels):
         first = torch.autograd.grad(y, ts, gy, retain_graph=True)
         again = torch.autograd.grad(y, ts, gy)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_a_tangent_is_refused():
+    """Forward mode, with and without a reverse-mode gradient as well: refused before the device is
+    looked at."""
+    import torch.autograd.forward_ad as fwd
+    from visionseg import _lib as L
+    t = L.tops()
+    x, r, w, b = torch.randn(3, 40), torch.randn(3, 40), torch.ones(40), torch.zeros(40)
+    for grad in (False, True):
+        with fwd.dual_level():
+            def dual(v):
+                return fwd.make_dual(v.clone().requires_grad_(grad), torch.ones_like(v))
+            for call in (lambda: t.gelu_act8(dual(x)), lambda: t.layer_norm_act8(dual(x), w, b, 1e-5),
+                         lambda: t.layer_norm_act8(x, dual(w), b, 1e-5), lambda: t.layer_norm_act8(x, w, dual(b), 1e-5),
+                         lambda: t.add_layer_norm_act8(dual(x), r, w, b, 1e-5),
+                         lambda: t.add_layer_norm_act8(x, dual(r), w, b, 1e-5)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()

@@ -33,3 +33,33 @@ def test_a_second_backward_over_a_retained_graph(dtype, T):
         first = torch.autograd.grad(y, ts, gy, retain_graph=True)
         again = torch.autograd.grad(y, ts, gy)
         assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from visionseg import _lib as L, ops
+    from visionseg.linear import linear_act8, mlp_act8
+    t = L.tops()
+    x, r, w, b = _rand((6, 40), F32, 1), _rand((6, 40), F32, 2), _rand((40,), F32, 3), _rand((40,), F32, 4)
+    wl = _rand((24, 40), F32, 5).requires_grad_()
+    wb = _rand((40, 24), F32, 6)
+    q, s = ops.act8_pack(x)
+    mean, rstd = _rand((6,), F32, 7), _rand((6,), F32, 8)
+    for grad in (False, True):
+        with fwd.dual_level():
+            def dual(v):
+                return fwd.make_dual(v.detach().clone().requires_grad_(grad), torch.ones_like(v))
+            for call in (lambda: ops.gelu_act8(dual(x)), lambda: ops.layer_norm_act8(dual(x), w, b),
+                         lambda: ops.layer_norm_act8(x, dual(w), b), lambda: ops.layer_norm_act8(x, w, dual(b)),
+                         lambda: ops.add_layer_norm_act8(dual(x), r, w, b),
+                         lambda: ops.add_layer_norm_act8(x, dual(r), w, b),
+                         lambda: ops.act8_wgrad(dual(x), q, s, 40, F32), lambda: t.act8_gelu_bwd(dual(x), q, s),
+                         lambda: t.act8_layer_norm_bwd(dual(x), None, q, s, w, mean, rstd),
+                         lambda: t.act8_layer_norm_bwd(x, dual(r), q, s, w, mean, rstd),
+                         lambda: linear_act8(dual(x), wl), lambda: mlp_act8(dual(x), wl, None, wb, None)):
+                with pytest.raises(RuntimeError, match="forward-mode|forward mode|jvp"):
+                    call()
+    # a tangent of the gradient that arrives
+    y = ops.gelu_act8(x.clone().requires_grad_())
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        y.backward(fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))

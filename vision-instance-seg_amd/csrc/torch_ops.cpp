@@ -477,6 +477,14 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> t
     TORCH_CHECK(t->device() == a.device(), "tensors on different devices: ", a.device(), " and ", t->device());
 }
 
+// No op here has a forward-mode derivative: a tangent is refused, not dropped.  (A C++ autograd
+// Function refuses it by itself; a call that keeps nothing does not pass through one.)
+void no_tangent(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->_fw_grad(0).defined(),
+                "8-bit activation checkpoints: no forward-mode derivative (an input carries a tangent)");
+}
+
 // x as rows of its last dimension: unit feature stride, any row stride
 at::Tensor as_rows(const at::Tensor& x, const char* what) {
   TORCH_CHECK(x.dim() >= 1, what, " must have at least one dimension");
@@ -539,6 +547,7 @@ at::Tensor act8_unpack(const at::Tensor& q, const at::Tensor& scale, int64_t fea
 
 // -> (gelu(x), q, scale); keep false: empty q, scale
 std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_gelu_fwd(const at::Tensor& x, bool keep) {
+  no_tangent({&x});
   on_device({&x});
   TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
   const c10::DeviceGuard guard(x.device());
@@ -556,6 +565,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_gelu_fwd(const at::Tensor& x
 // -> (gx, gelu(h) or an empty tensor)
 std::tuple<at::Tensor, at::Tensor> act8_gelu_bwd(const at::Tensor& grad_y, const at::Tensor& q, const at::Tensor& scale,
                                                  bool recompute) {
+  no_tangent({&grad_y});
   same_device(grad_y, {&q, &scale});
   TORCH_CHECK(grad_y.dim() >= 1, "grad_y must have at least one dimension");
   const int64_t C = grad_y.size(-1), rows = check_checkpoint(q, scale, C);
@@ -583,6 +593,8 @@ const int* row_map(const std::optional<at::Tensor>& rows, const at::Tensor& like
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> act8_layer_norm_fwd(
     const at::Tensor& x, const std::optional<at::Tensor>& r, const at::Tensor& weight, const at::Tensor& bias,
     double eps, const std::optional<at::Tensor>& rows, int64_t out_rows, bool keep) {
+  no_tangent({&x, &weight, &bias});
+  if (r.has_value()) no_tangent({&*r});
   same_device(x, {&weight, &bias});
   TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
   const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
@@ -617,6 +629,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
 std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_layer_norm_bwd(
     const at::Tensor& grad_y, const std::optional<at::Tensor>& grad_s, const at::Tensor& q, const at::Tensor& scale,
     const at::Tensor& weight, const at::Tensor& mean, const at::Tensor& rstd, const std::optional<at::Tensor>& rows) {
+  no_tangent({&grad_y, &weight, &mean, &rstd});
+  if (grad_s.has_value()) no_tangent({&*grad_s});
   same_device(grad_y, {&q, &scale, &weight, &mean, &rstd});
   TORCH_CHECK(weight.dim() == 1, "weight must be one-dimensional");
   const int64_t C = weight.size(0), M = check_checkpoint(q, scale, C);
@@ -651,6 +665,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_layer_norm_bwd(
 // -> (dw [N, features], db [N] or an empty tensor) in `dtype`
 std::tuple<at::Tensor, at::Tensor> act8_wgrad(const at::Tensor& grad_y, const at::Tensor& q, const at::Tensor& scale,
                                               int64_t features, at::ScalarType dtype, bool bias) {
+  no_tangent({&grad_y});
   same_device(grad_y, {&q, &scale});
   TORCH_CHECK(features >= 1, "act8_wgrad: at least one feature");
   const int64_t T = check_checkpoint(q, scale, features);
