@@ -1,0 +1,69 @@
+"""GPU tests of the weight gradient from 8-bit checkpoints, to the last bit, on every output tile of
+csrc/act8_wgrad.hip with and without splits of the tokens and in every way it reads a gradient."""
+import pytest
+import torch
+
+import _act8exact as ex
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+
+# T, K, N.  An odd N: bf16 rows that begin inside a dword
+BF16_SIZES = [
+    (65, 129, 127), (400, 256, 256), (5000, 64, 40), (100000, 20, 18), (100000, 20, 19),       # 64 x 64
+    (130, 1030, 2048), (130, 1030, 2047), (4000, 4100, 96), (200000, 96, 96), (200000, 96, 95),  # 128 x 128
+    (200, 4100, 1030), (200, 4100, 1031), (4000, 4100, 130), (4000, 4100, 131), (16384, 96, 2047),  # 256 x 128
+    (200, 4100, 2048), (200, 4100, 2047), (4001, 4100, 516), (4001, 4100, 515)]                 # 256 x 256
+F32_SIZES = [
+    (65, 130, 130), (1000, 96, 96), (10007, 203, 299), (150000, 20, 18),                   # 64 x 64
+    (130, 1030, 2047), (4000, 96, 2047), (2000, 4100, 96),                                      # 128 x 128
+    (200, 1030, 4100), (4000, 130, 2047), (9000, 2048, 96)]                                     # 128 x 256
+
+
+def _check(gy, q, scale, dw, db, K):
+    from visionseg import ops
+    for out in (F32, BF16):
+        gw, gb = ops.act8_wgrad(gy, q, scale, K, out, bias=True)
+        ex.same(gw, dw, "dw")
+        ex.same(gb, db, "db")
+        ex.same(ops.act8_wgrad(gy, q, scale, K, out), dw, "dw without db")
+
+
+@pytest.mark.parametrize("T,K,N,dtype", [(*s, BF16) for s in BF16_SIZES] + [(*s, F32) for s in F32_SIZES])
+def test_whole_numbers(T, K, N, dtype):
+    _check(*ex.whole(T, N, K, dtype, T + K + N, DEV), K)
+
+
+@pytest.mark.parametrize("T,K,N", F32_SIZES)
+def test_three_parts(T, K, N):
+    _check(*ex.parts(T, N, K, T + K + N, DEV), K)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,K,N,pitch,first", [
+    (200, 4100, 2047, 2049, 1), (200, 4100, 2048, 2051, 3), (130, 1030, 2047, 2048, 1), (4000, 130, 2047, 2047, 1),
+    (400, 256, 256, 263, 5)])
+def test_row_starts(T, K, N, pitch, first, dtype):
+    """Rows that begin anywhere in a wider buffer of NaN."""
+    for gy, q, scale, dw, db in (ex.whole(T, N, K, dtype, 1, DEV),) + ((ex.parts(T, N, K, 2, DEV),) if dtype == F32 else ()):
+        flat = torch.full((first + (T - 1) * pitch + N,), float("nan"), device=DEV, dtype=dtype)
+        rows = flat.as_strided((T, N), (pitch, 1), first)
+        rows.copy_(gy)
+        _check(rows, q, scale, dw, db, K)
+
+
+@pytest.mark.parametrize("T,K,N", [(70, 100, 40), (70, 1030, 2047), (70, 4100, 1030)])
+def test_rows_far_apart(T, K, N):
+    """64 rows that span more than 2^31 bytes, on each kind of tile."""
+    pitch = 1 << 24
+    gy, q, scale, dw, db = ex.whole(T, N, K, BF16, 3, DEV)
+    rows = torch.empty((T - 1) * pitch + N, device=DEV, dtype=BF16).as_strided((T, N), (pitch, 1))
+    rows.copy_(gy)
+    _check(rows, q, scale, dw, db, K)
+    del rows
+    gy, q, scale, dw, db = ex.parts(T, N, K, 4, DEV)
+    rows = torch.empty((T - 1) * pitch + N, device=DEV).as_strided((T, N), (pitch, 1))
+    rows.copy_(gy)
+    _check(rows, q, scale, dw, db, K)
