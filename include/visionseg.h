@@ -285,7 +285,8 @@ VS_API int vs_gelu_row_quantize_fp8(const void* h, void* y, void* q, float* scal
  *                               127 * 2^121, an infinity or a NaN (q 0) and stands for NaN
  * It stands for q * 2^e, which bf16 holds exactly.  Rows and features may be 0 (nothing is done)
  * and features need not be a multiple of anything; data pointers only need their element's
- * alignment. */
+ * alignment.  pack, unpack and GELU take up to 2^35 - 2048 elements, the padding counted, and refuse
+ * more. */
 /* x [rows, features] (dtype; row stride ld_x elements, unit feature stride) -> q, scale. */
 VS_API int vs_act8_pack(int dtype, const void* x, long long ld_x, void* q, void* scale, long long rows, int features,
                         void* stream);

@@ -57,3 +57,15 @@ def test_a_tangent_is_refused():
                          lambda: t.add_layer_norm_act8(x, dual(r), w, b, 1e-5)):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call()
+
+
+@pytest.mark.parametrize("rows,C", [(1 << 27, 256), ((1 << 27) - 7, 250), (1 << 32, 1), (33, 1 << 30), ((1 << 30) + 1, 32)])
+def test_tensors_beyond_one_launch_are_refused(rows, C):
+    """2^32 threads or more: refused before any HIP call, by name."""
+    import ctypes
+    from visionseg import _lib as L
+    lib, p = L.lib(), ctypes.c_void_p(16)
+    for rc in (lib.vs_act8_pack(1, p, C, p, p, rows, C, None), lib.vs_act8_unpack(1, p, p, p, rows, C, None),
+               lib.vs_act8_gelu_forward(1, p, p, p, p, rows, C, None),
+               lib.vs_act8_gelu_backward(1, p, p, p, p, p, rows, C, None)):
+        assert rc == -1 and b"too large" in lib.vs_last_error()

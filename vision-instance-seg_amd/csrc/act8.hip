@@ -21,17 +21,9 @@ struct Place {
   long long row;
   int j;
 };
-__device__ __forceinline__ Place place_of(long long g, int cpr, bool narrow) {
-  Place p;
-  if (narrow) {                                  // fewer than 2^32 chunks: a 32-bit division
-    const uint32_t r = (uint32_t)g / (uint32_t)cpr;
-    p.row = r;
-    p.j = (int)((uint32_t)g - r * (uint32_t)cpr);
-  } else {
-    p.row = g / cpr;
-    p.j = (int)(g - p.row * cpr);
-  }
-  return p;
+__device__ __forceinline__ Place place_of(long long g, int cpr) {
+  const uint32_t r = (uint32_t)g / (uint32_t)cpr;              // (fewer than 2^32 chunks)
+  return {(long long)r, (int)((uint32_t)g - r * (uint32_t)cpr)};
 }
 
 template <typename T, bool FLAT>
@@ -58,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) act8_fwd_kernel(const T* __restrict_
   const long long g = (long long)blockIdx.x * kThreads + threadIdx.x;
   if (g >= chunks) return;                       // (chunks is a multiple of 4: quads leave whole)
   Place pl = {};
-  if (!FLAT) pl = place_of(g, cpr, chunks < (1ll << 32));
+  if (!FLAT) pl = place_of(g, cpr);
   Chunk<T> c;
   load_at<T, FLAT>(c, x, ld, g, pl, C);
   float v[8];
@@ -87,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) act8_bwd_kernel(const T* __restrict_
   const uint2 b = *reinterpret_cast<const uint2*>(q + 8 * g);
   const uint32_t sb = scale[g >> 2];
   Place pl = {};
-  if (!FLAT) pl = place_of(g, cpr, chunks < (1ll << 32));
+  if (!FLAT) pl = place_of(g, cpr);
   Chunk<T> c;
   float h[8];
   if (MODE == 0) {
@@ -134,10 +126,11 @@ int check_tensor(const char* who, int dtype, long long rows, int features, const
   if (rows < 0 || features < 0 || features > (1 << 30)) return no("rows >= 0, 0 <= features <= 2^30");
   if (((uintptr_t)q & 7) != 0) return no("q must be 8-B aligned");
   const int cpr = padded32(features) / 8;
-  if (cpr && rows > (1ll << 39) / cpr) return no("tensor too large");
+  // a launch has fewer than 2^32 threads, whole workgroups of them
+  if (cpr && rows > ((1ll << 32) - kThreads) / cpr) return no("tensor too large (2^35 elements with the padding)");
   chunks = rows * cpr;
   groups = (chunks + kThreads - 1) / kThreads;
-  return groups < (1ll << 31) ? VS_OK : no("tensor too large");
+  return VS_OK;
 }
 
 template <typename T, int MODE>
