@@ -63,3 +63,26 @@ def test_tangents_are_refused():
     y = ops.gelu_act8(x.clone().requires_grad_())
     with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         y.backward(fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linears_of_no_inputs_or_outputs(dtype):
+    """What F.linear gives, gradients too."""
+    import torch.nn.functional as F
+    from visionseg.linear import linear_act8, mlp_act8
+
+    def plain_mlp(x, w1, b1, w2, b2):
+        return F.linear(F.gelu(F.linear(x, w1, b1)), w2, b2)
+
+    def compare(fn, plain, shapes):
+        ts = [_rand(s, dtype, k).requires_grad_() for k, s in enumerate(shapes)]
+        got, want = fn(*ts), plain(*ts)
+        assert got.shape == want.shape and torch.equal(got, want)
+        for a, b in zip(torch.autograd.grad(got.sum(), ts, allow_unused=True),
+                        torch.autograd.grad(want.sum(), ts, allow_unused=True)):
+            assert (a is None) == (b is None) and (a is None or (a.shape == b.shape and torch.equal(a, b)))
+
+    for T, K, N in ((0, 40, 24), (5, 0, 24), (5, 40, 0), (0, 0, 3), (0, 3, 0)):
+        compare(linear_act8, F.linear, ((T, K), (N, K), (N,)))
+    for T, C, H, O in ((0, 40, 24, 8), (5, 0, 24, 8), (5, 40, 0, 8), (5, 40, 24, 0)):
+        compare(mlp_act8, plain_mlp, ((T, C), (H, C), (H,), (O, H), (O,)))

@@ -1067,9 +1067,9 @@ class _MlpAct8Fn(torch.autograd.Function):
 
 def _act8_ready(x, *params) -> bool:
     """Whether an act8 Function takes these: a device tensor that a gradient is wanted of, all
-    in one dtype of the kernels'."""
+    in one dtype of the kernels', no layer without inputs or outputs."""
     return (x.is_cuda and torch.is_grad_enabled() and x.dtype in (torch.float32, torch.bfloat16)
-            and all(p is None or p.dtype == x.dtype for p in params))
+            and all(p is None or (p.dtype == x.dtype and p.numel() > 0) for p in params))
 
 
 def linear_act8(x, w, b=None):
