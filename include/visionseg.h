@@ -54,6 +54,8 @@ enum vs_status { VS_OK = 0, VS_ERR_INVALID = -1, VS_ERR_HIP = -2, VS_ERR_UNSUPPO
 
 VS_API int vs_abi_version(void);
 VS_API const char* vs_last_error(void);
+/* The capture that `stream` is recording into (0: none; no two captures of a process share one). */
+VS_API unsigned long long vs_stream_capture_id(void* stream);
 
 /* ---- a8: multi-scale deformable attention sampling -------------------------------
  * value       [B, S, H, 32]            dtype      (S = sum_l H_l*W_l, head dim 32)

@@ -27,6 +27,7 @@ _P = _c_void_p
 # name -> argtypes (restype int unless noted); keep in sync with include/visionseg.h
 SIGNATURES = {
     "vs_abi_version": [],
+    "vs_stream_capture_id": [_P],
     "vs_last_error": [],
     "vs_msda_forward": [_c_int, _P, _P, _P, _P, _P, _P] + [_c_int] * 7 + [_P],
     "vs_msda_backward": [_c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P] + [_c_int] * 7 + [_P],
@@ -140,7 +141,8 @@ SIGNATURES = {
     "vs_conv3x3_wgrad_workspace_bytes": [_c_int] * 5,
     "vs_conv3x3_wgrad": [_c_int, _P, _P, _P, _P] + [_c_int] * 5 + [_P],
 }
-RESTYPES = {"vs_last_error": ctypes.c_char_p, "vs_masked_attn_workspace_bytes": ctypes.c_longlong,
+RESTYPES = {"vs_last_error": ctypes.c_char_p, "vs_stream_capture_id": ctypes.c_ulonglong,
+            "vs_masked_attn_workspace_bytes": ctypes.c_longlong,
             "vs_mask_head_backward_workspace_bytes": ctypes.c_longlong,
             "vs_layer_norm_backward_workspace_bytes": ctypes.c_longlong,
             "vs_column_sum_workspace_bytes": ctypes.c_longlong,

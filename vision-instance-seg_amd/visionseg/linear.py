@@ -21,6 +21,7 @@ from . import ops
 
 import ctypes
 import os
+import weakref
 
 # Linears over at least this many tokens take the token path (_LinearFn: the token GEMM where
 # its shape rule picks it, token_wgrad with the fused bias column sums, residual sinks).  4096
@@ -177,44 +178,67 @@ def _dgrad_on_token_gemm(T: int, weight, dtype) -> bool:
             and N % 8 == 0 and T >= MIN_TOKENS and _use_token_gemm_dgrad(T, K, N))
 
 
+class _Transpose:
+    """One Linear's request for W^T [K, N] (its autograd context holds it); place: where it was
+    made (_place)."""
+    __slots__ = ("weight", "out", "place", "done", "__weakref__")
+
+    def __init__(self, weight, place):
+        self.weight, self.place, self.done = weight, place, False
+        self.out = torch.empty(weight.shape[1], weight.shape[0], device=weight.device, dtype=weight.dtype)
+
+
+def _place(weight):
+    """Where work on weight goes now: the device, its current stream and, while that stream
+    captures, the capture."""
+    s = torch.cuda.current_stream(weight.device).cuda_stream
+    return weight.device, s, L.lib().vs_stream_capture_id(s)
+
+
 class _WeightTransposes:
     """W^T [K, N] copies of the token Linears' weights for the dX GEMM on the token GEMM
     (whose operands are both K-contiguous rows): requested in the forward (request), all
     written by ONE batched launch (ops.transpose_batched) at the first use in the backward
     (get).  Before, each dX GEMM made its own weight.t().contiguous(): 53 strided-copy
     launches per C2 step (0.33 ms, profiles/r6_glue_c2.txt).  The weights do not change
-    between a forward and its backward (the optimizer steps after).  A request never used
-    (a forward without backward) is dropped after `cap` newer ones; get() then falls back to
-    its own copy."""
+    between a forward and its backward (the optimizer steps after).
 
-    def __init__(self, cap: int = 1024):
-        self.pending = []
-        self.cap = cap
+    A launch takes the requests of its own place only: on another stream nothing would order it
+    before their use, and a captured one runs at replays alone, when what was requested outside
+    that capture has long been read or freed.  A request is held by its forward's autograd context
+    and by nothing else, so a forward without a backward leaves none behind.  A backward that
+    finds itself elsewhere than its forward makes a copy of its own."""
+
+    def __init__(self):
+        self.live = {}                        # place -> its unwritten requests, oldest first
+        self.count = 0
+
+    @property
+    def pending(self):
+        return [h for hs in list(self.live.values()) for h in list(hs.values())]
 
     def request(self, weight):
-        h = [weight, torch.empty(weight.shape[1], weight.shape[0], device=weight.device, dtype=weight.dtype), False]
-        self.pending.append(h)
-        if len(self.pending) > self.cap:
-            self.pending.pop(0)
+        h = _Transpose(weight, _place(weight))
+        if h.place not in self.live:
+            self.live = {k: hs for k, hs in self.live.items() if len(hs)}
+            self.live[h.place] = weakref.WeakValueDictionary()
+        self.count += 1
+        self.live[h.place][self.count] = h
         return h
 
-    def flush(self):
-        by_dev = {}
-        for h in self.pending:
-            by_dev.setdefault(h[0].device, []).append(h)
-        for hs in by_dev.values():
-            ops.transpose_batched([(h[0].detach().contiguous(), h[1]) for h in hs])
-            for h in hs:
-                h[2] = True
-        self.pending = []
+    def flush(self, place):
+        hs = list(self.live.pop(place, {}).values())
+        ops.transpose_batched([(h.weight.detach().contiguous(), h.out) for h in hs])
+        for h in hs:
+            h.done = True
 
     def get(self, h):
-        if not h[2]:
-            if any(p is h for p in self.pending):
-                self.flush()
-            else:                     # dropped: a copy of its own
-                return h[0].t().contiguous()
-        return h[1]
+        if h.place == _place(h.weight):
+            if not h.done:
+                self.flush(h.place)
+            if h.done:
+                return h.out
+        return h.weight.t().contiguous()
 
 
 _WT = _WeightTransposes()
