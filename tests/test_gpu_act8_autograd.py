@@ -86,3 +86,42 @@ def test_linears_of_no_inputs_or_outputs(dtype):
         compare(linear_act8, F.linear, ((T, K), (N, K), (N,)))
     for T, C, H, O in ((0, 40, 24, 8), (5, 0, 24, 8), (5, 40, 0, 8), (5, 40, 24, 0)):
         compare(mlp_act8, plain_mlp, ((T, C), (H, C), (H,), (O, H), (O,)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_kernel_timer_books_what_is_moved(dtype):
+    """bench's kernel table: every op's forward and backward is timed, with its algorithmic bytes."""
+    from visionseg import ops
+    from visionseg.linear import mlp_act8
+    from visionseg.profiling import KernelTimer
+    T, C, N, e = 70, 40, 24, dtype.itemsize
+    n, ck = T * C, T * (64 + 2)
+    x, r = _rand((T, C), dtype, 1).requires_grad_(), _rand((T, C), dtype, 2).requires_grad_()
+    w, b = _rand((C,), dtype, 3).requires_grad_(), _rand((C,), dtype, 4)
+    gy = _rand((T, N), dtype, 5)
+    w1, w2 = _rand((N, C), dtype, 6).requires_grad_(), _rand((C, N), dtype, 7).requires_grad_()
+    with KernelTimer() as t:
+        q, s = ops.act8_pack(x.detach())
+        ops.act8_unpack(q, s, C, dtype)
+        ops.act8_wgrad(gy, q, s, C, F32, bias=True)
+        ops.gelu_act8(x).sum().backward()
+        ops.layer_norm_act8(x, w, b).sum().backward()
+        ops.add_layer_norm_act8(x, r, w, b)[1].sum().backward()
+    with KernelTimer() as m:
+        mlp_act8(x, w1, None, w2, None).sum().backward()
+    with torch.no_grad(), KernelTimer() as f:
+        ops.gelu_act8(x)
+    ops.gelu_act8(x).sum().backward()                        # no timer: nothing is booked
+    torch.cuda.synchronize()
+    want = {"act8_pack": n * e + ck, "act8_unpack": n * e + ck, "act8_wgrad": T * N * e + ck + N * C * 4,
+            "gelu_act8": 2 * n * e + ck, "gelu_act8_bwd": 2 * n * e + ck,
+            "layer_norm_act8": 2 * n * e + ck, "layer_norm_act8_bwd": 2 * n * e + ck,
+            "add_layer_norm_act8": 4 * n * e + ck, "add_layer_norm_act8_bwd": 3 * n * e + ck}
+    got = t.summary()
+    assert {k: v["bytes"] for k, v in got.items()} == want
+    assert all(v["launches"] == 1 and v["total_ms"] > 0 for v in got.values())
+    assert got["act8_wgrad"]["flops"] == 2 * T * N * C
+    hk = T * (32 + 1)
+    got = m.summary()
+    assert got["act8_gelu_fwd"]["bytes"] == 2 * T * N * e + hk and got["act8_gelu_bwd"]["bytes"] == 3 * T * N * e + hk
+    assert {k: v["bytes"] for k, v in f.summary().items()} == {"gelu_act8": 2 * n * e}

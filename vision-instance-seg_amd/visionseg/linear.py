@@ -1054,7 +1054,7 @@ class _MlpAct8Fn(torch.autograd.Function):
         K = x.shape[-1]
         # (a frozen fc1 needs nothing of x)
         q, scale = ops.act8_pack(x.reshape(-1, K)) if ctx.needs_input_grad[1] else (None, None)
-        h, hq, hs = ops._act8()["act8_gelu_fwd"](_forward_gemm(x, w1, b1).reshape(-1, w1.shape[0]), True)
+        h, hq, hs = ops._act8_gelu_fwd(_forward_gemm(x, w1, b1).reshape(-1, w1.shape[0]))
         ctx.save_for_backward(q, scale, hq, hs, w1, w2)
         ctx.shape, ctx.has_bias = x.shape, (b1 is not None, b2 is not None)
         T, need = h.shape[0], ctx.needs_input_grad
@@ -1068,7 +1068,7 @@ class _MlpAct8Fn(torch.autograd.Function):
         q, scale, hq, hs, w1, w2 = ctx.saved_tensors
         need = ctx.needs_input_grad
         gy2 = gy.reshape(-1, gy.shape[-1]).to(w2.dtype)
-        gh, h = ops._act8()["act8_gelu_bwd"](_dgrad_gemm(gy2, w2, ctx.wt[1]), hq, hs, need[3])
+        gh, h = ops._act8_gelu_bwd(_dgrad_gemm(gy2, w2, ctx.wt[1]), hq, hs, need[3])
         gw1 = gb1 = gw2 = gb2 = None
         if need[3]:
             if ctx.has_bias[1] and need[4]:

@@ -26,7 +26,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .profiling import enabled as profiling_enabled
-from .profiling import timed
+from .profiling import timed, timed_backward
 
 
 def _shapes_list(spatial_shapes):
@@ -1564,28 +1564,56 @@ def _act8():
     return _ACT8
 
 
-def _act8_call(name, like, tensors, checkpoints, *args, flops=0):
-    """The op on args; its forward timed where a KernelTimer is active, as `tensors` passes over a
-    tensor like `like` and `checkpoints` over its checkpoint."""
+def _checkpoint_bytes(rows: int, features: int) -> int:
+    P = (features + 31) // 32 * 32
+    return rows * (P + P // 32)
+
+
+def _act8_call(name, like, work, *args):
+    """The op on args, timed where a KernelTimer is active; work() -> (its bytes, its flops)."""
     op = _act8()[name]
     if not profiling_enabled():
         return op(*args)
-    n = like.numel()
-    with timed(name, like, bytes_=n * (tensors * like.element_size() + checkpoints), flops=float(n * flops)):
+    bytes_, flops = work()
+    with timed(name, like, bytes_=bytes_, flops=flops):
         return op(*args)
+
+
+def _act8_kept(name, x, tensors, *args):
+    """The op on args that keeps x's checkpoint where a gradient is wanted: its forward, which reads
+    and writes `tensors` tensors like x, and its backward (gy -- and gs, of a residual norm -- in, gx
+    out) timed where a KernelTimer is active."""
+    op = _act8()[name]
+    if not profiling_enabled():
+        return op(*args)
+    n, C = x.numel(), max(1, x.shape[-1])
+    kept = _checkpoint_bytes(n // C, C)
+    grad = torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args)
+    with timed(name, x, bytes_=n * tensors * x.element_size() + (kept if grad else 0)):
+        out = op(*args)
+    timed_backward(name + "_bwd", out[0] if isinstance(out, (tuple, list)) else out,
+                   n * (2 if tensors == 2 else 3) * x.element_size() + kept)
+    return out
 
 
 def act8_pack(x):
     """x [..., C] (f32 / bf16; a 2-D x may have any row stride) -> (q, scale)."""
     L.require_hip(x)
-    return _act8_call("act8_pack", x, 1, 1, x)
+
+    def work():
+        rows = x.numel() // max(1, x.shape[-1])
+        return x.numel() * x.element_size() + _checkpoint_bytes(rows, x.shape[-1]), 0.0
+    return _act8_call("act8_pack", x, work, x)
 
 
 def act8_unpack(q, scale, features: int, dtype):
     """The values [..., features] that a checkpoint stands for, in dtype (f32 / bf16: both
     exact)."""
     L.require_hip(q, scale)
-    return _act8_call("act8_unpack", q, 3, 0, q, scale, features, dtype)
+
+    def work():
+        return q.numel() + scale.numel() + q.numel() // max(1, q.shape[-1]) * features * dtype.itemsize, 0.0
+    return _act8_call("act8_unpack", q, work, q, scale, features, dtype)
 
 
 def act8_wgrad(gy, q, scale, features: int, out_dtype, bias: bool = False):
@@ -1594,15 +1622,33 @@ def act8_wgrad(gy, q, scale, features: int, out_dtype, bias: bool = False):
     (dW, db) with db [N] = the column sums of gy.  Exact products, f32 accumulation
     (csrc/act8_wgrad.hip; the uncompressed form is token_wgrad)."""
     L.require_hip(gy, q, scale)
-    dw, db = _act8_call("act8_wgrad", gy, 1, 0, gy, q, scale, features, out_dtype, bias, flops=2 * features)
+
+    def work():
+        return (gy.numel() * gy.element_size() + q.numel() + scale.numel() + gy.shape[-1] * features * out_dtype.itemsize,
+                2.0 * gy.numel() * features)
+    dw, db = _act8_call("act8_wgrad", gy, work, gy, q, scale, features, out_dtype, bias)
     return (dw, db) if bias else dw
+
+
+def _act8_gelu_fwd(x):
+    """(gelu(x), q, scale) for a contiguous x, with no autograd of its own."""
+    def work():
+        return 2 * x.numel() * x.element_size() + _checkpoint_bytes(x.numel() // x.shape[-1], x.shape[-1]), 0.0
+    return _act8_call("act8_gelu_fwd", x, work, x, True)
+
+
+def _act8_gelu_bwd(gy, q, scale, recompute: bool):
+    """(gy gelu'(h), gelu(h) or an empty tensor) for the checkpoint's h."""
+    def work():
+        return (3 if recompute else 2) * gy.numel() * gy.element_size() + q.numel() + scale.numel(), 0.0
+    return _act8_call("act8_gelu_bwd", gy, work, gy, q, scale, recompute)
 
 
 def gelu_act8(x):
     """F.gelu(x) (exact) for x [..., C] f32 / bf16, whose backward reads x's 8-bit checkpoint
     instead of x: dx = dy (Phi(h) + h phi(h)) at the checkpointed h (once differentiable)."""
     L.require_hip(x)
-    return _act8_call("gelu_act8", x, 2, 1, x)
+    return _act8_kept("gelu_act8", x, 2, x)
 
 
 def layer_norm_act8(x, weight, bias, eps: float = 1e-5, wrows=None):
@@ -1612,8 +1658,8 @@ def layer_norm_act8(x, weight, bias, eps: float = 1e-5, wrows=None):
     LayerNormFunction)."""
     L.require_hip(x, weight, bias)
     if wrows is None:
-        return _act8_call("layer_norm_act8", x, 2, 1, x, weight, bias, eps)
-    return _act8_call("layer_norm_act8", x, 2, 1, x, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
+        return _act8_kept("layer_norm_act8", x, 2, x, weight, bias, eps)
+    return _act8_kept("layer_norm_act8", x, 2, x, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
 
 
 def add_layer_norm_act8(x, r, weight, bias, eps: float = 1e-5, wrows=None):
@@ -1621,8 +1667,8 @@ def add_layer_norm_act8(x, r, weight, bias, eps: float = 1e-5, wrows=None):
     (see layer_norm_act8)."""
     L.require_hip(x, r, weight, bias)
     if wrows is None:
-        return _act8_call("add_layer_norm_act8", x, 4, 1, x, r, weight, bias, eps)
-    return _act8_call("add_layer_norm_act8", x, 4, 1, x, r, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
+        return _act8_kept("add_layer_norm_act8", x, 4, x, r, weight, bias, eps)
+    return _act8_kept("add_layer_norm_act8", x, 4, x, r, weight, bias, eps, wrows.rows, wrows.pad, wrows.total)
 
 
 # ------------------------------------------------------------------ per-parameter clip

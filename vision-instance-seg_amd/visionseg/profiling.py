@@ -75,3 +75,22 @@ def timed(name: str, like: torch.Tensor, bytes_: float = 0.0, flops: float = 0.0
     finally:
         b.record(s)
         t.events[name].append((a, b, float(bytes_), float(flops)))
+
+
+def timed_backward(name: str, y: torch.Tensor, bytes_: float = 0.0):
+    """Bracket the backward of the autograd node that made y (one whose launches run in C++), each
+    time it runs while a timer is active."""
+    if _active is None or y.grad_fn is None:
+        return
+    like, running = y.new_empty(0), []
+
+    def before(grads):
+        running.append(timed(name, like, bytes_))
+        running[-1].__enter__()
+
+    def after(grads_in, grads_out):
+        if running:
+            running.pop().__exit__(None, None, None)
+
+    y.grad_fn.register_prehook(before)
+    y.grad_fn.register_hook(after)
