@@ -285,7 +285,7 @@ VS_API int vs_gelu_row_quantize_fp8(const void* h, void* y, void* q, float* scal
  *   q      int8  [rows, P]      P = C rounded up to a multiple of 32, zeros behind C; 8-B aligned
  *   scale  uint8 [rows, P / 32] e + 127 (1..248), or 255: the block held a magnitude above
  *                               127 * 2^121, an infinity or a NaN (q 0) and stands for NaN
- * It stands for q * 2^e, which bf16 holds exactly.  Rows and features may be 0 (nothing is done)
+ * It stands for q * 2^e, which bf16 holds exactly and which is off by at most max(a / 127, 2^-127).  Rows and features may be 0 (nothing is done)
  * and features need not be a multiple of anything; data pointers only need their element's
  * alignment.  pack, unpack and GELU take up to 2^35 - 2048 elements, the padding counted, and refuse
  * more. */
@@ -322,7 +322,8 @@ VS_API int vs_act8_layer_norm_backward(int dtype, const void* gy, const void* gs
  * outputs and K inputs from its output gradient gy [tokens, N] (dtype; row stride ld_gy >= N,
  * unit feature stride) and the checkpoint of its input (q 16-B aligned): dw [N, K], db [N] in
  * out_dtype (overwritten; 0 where tokens is 0).  f32 accumulation; bf16 gy: exact products;
- * f32 gy: exact products too (three bf16 parts).  K > 0.  Deterministic. */
+ * f32 gy: exact products too (three bf16 parts) where |gy| >= 2^-110, off by less than 2^-133 |h|
+ * below.  K > 0.  Deterministic. */
 VS_API long long vs_act8_wgrad_workspace_bytes(int dtype, long long tokens, int N, int K);
 VS_API int vs_act8_wgrad(int dtype, int out_dtype, const void* gy, long long ld_gy, const void* q, const void* scale,
                          void* dw, void* db, void* workspace, long long tokens, int N, int K, void* stream);

@@ -67,3 +67,37 @@ def test_rows_far_apart(T, K, N):
     rows = torch.empty((T - 1) * pitch + N, device=DEV).as_strided((T, N), (pitch, 1))
     rows.copy_(gy)
     _check(rows, q, scale, dw, db, K)
+
+
+def test_three_parts_down_to_denormals():
+    """A gradient of 2^-110 or more is the sum of its parts; below, bf16's last bit, 2^-133, is where they
+    are cut (towards zero: off by less than that, times |h|)."""
+    from visionseg import ops
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for he in (0, 20, -10):
+        q, scale = ops.act8_pack(torch.full((1, 32), 2.0 ** he, device=DEV))
+        for e in (-149, -140, -134, -133, -130, -127, -126, -120, -118, -112, -111, -110, -109, -104, -103, -96):
+            v = (torch.randint(1 << 23, 1 << 24, (1, 515), generator=g, device=DEV) | 1).double() * 2.0 ** (e - 23)
+            gy = v.float()                                   # (rounded below 2^-126)
+            dw = ops.act8_wgrad(gy, q, scale, 32, F32).double()
+            want = (gy.double() * 2.0 ** he).view(-1, 1).expand_as(dw)
+            if e >= -110:
+                assert torch.equal(dw, want), (he, e)
+            else:
+                # (and the result's own rounding where it is a denormal)
+                assert bool(((dw - want).abs() < 2.0 ** (he - 133) + (2.0 ** -150 if he < 0 else 0)).all()), (he, e)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_checkpoint_error_bound(dtype):
+    """At most 1 / 127 of the block's largest magnitude, or 2^-127."""
+    from visionseg import ops
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(4000, 64, generator=g, device=DEV, dtype=torch.float64)
+    x = (x * 2.0 ** torch.linspace(-148, 125, 4000, device=DEV, dtype=torch.float64).view(-1, 1)).to(dtype)
+    v = ops.act8_unpack(*ops.act8_pack(x), 64, F32).double()
+    a = x.double().view(4000, 2, 32).abs().amax(-1, keepdim=True)
+    off = (v - x.double()).view(4000, 2, 32).abs()
+    held = (a <= 127 * 2.0 ** 121).expand_as(off)            # above: NaN
+    assert bool((off <= torch.clamp(a / 127, min=2.0 ** -127))[held].all())
+    assert bool(torch.isnan(off[~held]).all())

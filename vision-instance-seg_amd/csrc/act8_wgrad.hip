@@ -3,10 +3,12 @@
 //
 // The reduction runs over tokens, the strided dimension of both operands: 64-token chunks are
 // staged in LDS in their natural [token][feature] order (images of 128 columns, padded row
-// pitches: kPitchG, kPitchX) and read as MFMA operands with the transposing LDS read.  The checkpoint is widened to bf16 on its
-// way into LDS, once a workgroup, exactly (act8.h).  f32 gradients are cut into three bf16 parts
-// by truncation, gY = hi + mid + lo: 8 bits of significand each, so the sum is exact, and three
-// matrix products give what an f32 product of exact terms would; a non-finite value is its hi
+// pitches: kPitchG, kPitchX) and read as MFMA operands with the transposing LDS read.  The
+// checkpoint is widened to bf16 on its way into LDS, once a workgroup, exactly (act8.h).  f32
+// gradients are cut into three bf16 parts by truncation, gY = hi + mid + lo: 8 bits of significand
+// each, so that the sum is exact for |gY| >= 2^-110 (bf16's last bit is 2^-133, which the matrix
+// units keep: below, what lies under it is cut, and a product is off by less than 2^-133 |h|), and
+// three matrix products give what an f32 product of exact terms would; a non-finite value is its hi
 // part alone.  Accumulation is f32 in the matrix units.  db is summed on the way into LDS, every
 // workgroup of an output block its share of the chunks.
 //
