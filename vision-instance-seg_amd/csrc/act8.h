@@ -178,8 +178,9 @@ __device__ __forceinline__ void unpack_chunk(uint2 q, uint32_t scale, float* v) 
 // The normal distribution's tail by its Mills ratio M(a) = (1 - Phi(a)) / phi(a), a >= 0: smooth,
 // falling from sqrt(pi / 2) like 1 / a, so t poly(t) with t = 1 / (1 + p a) fits it in RELATIVE
 // error (least squares with the weights raised where the error is largest, until it is level,
-// over 0 <= a <= 14.5): degree 6 to 9e-6 for bf16 results (half a step: 2e-3), degree 9 to 3.4e-8
-// for f32 ones.  gelu(x) and its slope then need one exponential and one reciprocal:
+// over 0 <= a <= 14.5): degree 6 to 9e-6 for bf16 results (half a step: 2e-3), degree 9 to 3.6e-8
+// for f32 ones (half a step: 6e-8; with the coefficients as rounded to f32, whose last bits were
+// searched for the smallest error).  gelu(x) and its slope then need one exponential and one reciprocal:
 //     gelu(x)  = max(x, 0) - |x| M(|x|) phi(x)
 //     gelu'(x) = [x >= 0] + sign(x) (|x| - M(|x|)) phi(x)
 template <typename T> struct Mills;
@@ -197,17 +198,22 @@ template <> struct Mills<bf16> {
 };
 template <> struct Mills<float> {
   __device__ __forceinline__ static float at(float a) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.34f, a, 1.f));
-    float s = -6.486242265e-02f;
-    s = fmaf(s, t, 3.468089104e-01f);
-    s = fmaf(s, t, -6.789714098e-01f);
+    // M moves 2.35 times as much as t near a = 0, so what the denominator's rounding and the
+    // reciprocal's leave, rho = 1 - (1 + p a) t, is taken back to first order: M(t + t rho) = M(t)
+    // (1 + g rho), g = t M'(t) / M(t), 1 at t = 0 and 2.35 at t = 1
+    const float d = fmaf(0.34f, a, 1.f), t = __builtin_amdgcn_rcpf(d);
+    const float rho = fmaf(-fmaf(0.34f, a, 1.f - d), t, fmaf(-d, t, 1.f));
+    float s = -6.486240029e-02f;
+    s = fmaf(s, t, 3.468088210e-01f);
+    s = fmaf(s, t, -6.789713502e-01f);
     s = fmaf(s, t, 5.006161928e-01f);
-    s = fmaf(s, t, -1.080504507e-01f);
-    s = fmaf(s, t, 2.875439823e-01f);
-    s = fmaf(s, t, 2.891439199e-01f);
+    s = fmaf(s, t, -1.080504805e-01f);
+    s = fmaf(s, t, 2.875439227e-01f);
+    s = fmaf(s, t, 2.891439795e-01f);
     s = fmaf(s, t, 3.411326110e-01f);
     s = fmaf(s, t, 3.399528861e-01f);
-    return s * t;
+    const float m = s * t;
+    return fmaf(m * fmaf(1.35f, t, 1.f), rho, m);
   }
 };
 
