@@ -125,3 +125,29 @@ def test_kernel_timer_books_what_is_moved(dtype):
     got = m.summary()
     assert got["act8_gelu_fwd"]["bytes"] == 2 * T * N * e + hk and got["act8_gelu_bwd"]["bytes"] == 3 * T * N * e + hk
     assert {k: v["bytes"] for k, v in f.summary().items()} == {"gelu_act8": 2 * n * e}
+
+
+def test_backbone_under_autocast():
+    """M2FConfig.act8 under autocast: the norms are the plain ones, the qkv projections and MLPs keep
+    8 bits (test_gpu_act8.test_swin_backbone has the bounds of the types without it)."""
+    from visionseg.model import M2FConfig, SwinBackbone
+    px = _rand((1, 3, 224, 256), F32, 1)
+    out = {}
+    for act8 in (False, True):
+        torch.manual_seed(0)
+        net = SwinBackbone(M2FConfig(embed_dim=96, depths=(2, 2), num_heads=(3, 6), window_size=7, act8=act8)).to(DEV)
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        with torch.autocast("cuda", torch.bfloat16):
+            feats = net(px)
+        kept = torch.cuda.memory_allocated() - base
+        grads = torch.autograd.grad(feats, list(net.parameters()), [_rand(f.shape, f.dtype, i) for i, f in enumerate(feats)])
+        out[act8] = (feats, grads, kept)
+    for a, c in zip(out[True][0], out[False][0]):
+        assert a.dtype == c.dtype
+        a, c = a.detach().double(), c.detach().double()
+        assert float((a - c).norm() / c.norm()) < 2e-2
+    for a, c in zip(out[True][1], out[False][1]):
+        assert a.dtype == c.dtype == F32
+        assert float((a.double() - c.double()).norm()) <= 0.05 * float(c.double().norm()) + 1e-12
+    assert out[True][2] < out[False][2]

@@ -865,7 +865,7 @@ class TokenLayerNorm(nn.LayerNorm):
         """LN(x) in the window layout of wrows (ops.WindowRows: the Swin partition folded
         into the kernel's stores) -> [wrows.total, C]; quant (bf16, C % 32 == 0): -> (y,
         (e4m3, e8m0 scales) of y) for an fp8 consumer, (y, None) where the copy cannot be made;
-        act8: the norm keeps its input in 8 bits (ops.layer_norm_act8)."""
+        act8: the norm keeps its input in 8 bits (ops.layer_norm_act8; see _act8_ok)."""
         if act8 and self._act8_ok(x):
             return ops.layer_norm_act8(x, self.weight, self.bias, self.eps, wrows=wrows)
         if self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight) \
@@ -881,6 +881,8 @@ class TokenLayerNorm(nn.LayerNorm):
         return (y, None) if quant else y
 
     def _act8_ok(self, x) -> bool:
+        """Whether the norm of x runs on the act8 kernels (under autocast, whose norm is torch's f32
+        one, it does not, and keeps x as it is)."""
         return (self.elementwise_affine and self.bias is not None and ops.layer_norm_supported(x, self.weight)
                 and not torch.is_autocast_enabled())
 
