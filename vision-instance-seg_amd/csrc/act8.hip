@@ -3,10 +3,11 @@
 //
 // One pass over the data each, a chunk a thread: loads, ~20-40 vector instructions an element and
 // stores, bound by memory.  Measured (a copy of 1 GiB runs at 5.15 TB/s): 262144 x 384 bf16, written
-// in 52 us (5.9 TB/s: part of it stays in the last-level cache) and read back in 52;  65536 x 2048
-// bf16, GELU forward 112 us (6.0 TB/s), backward 114 (5.9), with the activation again 161 (5.9);
-// 50021 x 201 f32, written in 9.6 us and read back in 12.1 (4.1).  Two or four chunks a thread, all
-// loaded before the first use, were no faster (GELU backward 122, 123 us).
+// in 52 us (5.9 TB/s: part of it stays in the last-level cache) and read back in 49;  65536 x 2048
+// bf16, GELU forward 107 us (6.3 TB/s), backward 114-122 (5.9-5.5), with the activation again 160
+// (5.9);  32768 x 2048 f32 (with the reciprocal's correction, act8.h; the same without), 105, 106 and
+// 160;  50021 x 201 f32, written in 9.1 us and read back in 11.2 (4.6).  Two or four chunks a thread,
+// all loaded before the first use, were no faster (GELU backward 122, 123 us where one took 114).
 #include "act8.h"
 
 namespace vs {

@@ -12,8 +12,10 @@
 // more than 2048 features take the whole workgroup (G = 256, one exchange through LDS).
 // Statistics are f32, the variance in a second pass over the registers.
 //
-// Measured: 589824 x 192 bf16 with the residual, forward 192 us (5.3 TB/s), backward 166 (4.8) + 5 for
-// the sum;  65536 x 768 bf16, 41 (6.1) and 51 (4.9);  4099 x 1003 f32, 10 (3.7) and 13 + 3.6 (2.8).
+// Measured: 589824 x 192 bf16 with the residual, forward 197 us (5.2 TB/s), backward 166 (4.8) + 5 for
+// the sum, in the window layout the same;  65536 x 768 bf16, 49 (5.2) and 49 + 4 (5.2);  4099 x 1003
+// f32, 14 (2.7) and 18 + 4 (2.1: four waves a CU ask for a row, wait for it and store before they ask for
+// the next), with the residual 17 (4.1) and 16.5 + 4 (3.2).
 //
 // dw / db: summed by every lane over the rows it sweeps, over the workgroup's groups in LDS,
 // written as one f32 row a workgroup and added up by a second kernel: a fixed order, no atomics.

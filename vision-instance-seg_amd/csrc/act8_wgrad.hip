@@ -19,13 +19,14 @@
 //
 // What bounds it.  Vector arithmetic costs MFMA time almost in full (64 idle instructions more a
 // chunk: 10 to 16 % more time), so the widening of the checkpoint, 2.5 instructions an element, is
-// what an uncompressed operand would save; at large sizes the clock falls to ~1.6 GHz with the matrix
-// units busy 68 % of the cycles.  Measured on several cards (they differ by up to 15 %):  147456
-// tokens x 1024 x 2048 bf16 540-595 us (1040-1145 TF/s; the library's 8192^3 product 1475, its
-// product at these sizes and layouts 570);  16384 x 1536 x 384 35-37 us, of it 7.7 for the sum of 14
-// splits (33 MB of partials; the products alone are 13 us at the library's rate);  262144 x 96 x 384
-// 44-47;  400 x 256 x 256 7 (seven chunks in a row);  f32 65536 x 768 x 768 210-250
-// (310-370 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 18.
+// what an uncompressed operand would save; at the largest size below the matrix units are busy
+// 64 to 67 % of the cycles and the clock falls from 1.8 to 1.5 GHz within four launches in a row.
+// Measured on several cards (they differ by up to 15 %), tokens x outputs x inputs:  147456 x 1024 x
+// 2048 bf16 530-610 us, 15 of it for the sum of the splits (1015-1165 TF/s; the library's 8192^3
+// product 1475, its product at these sizes and layouts 570);  16384 x 1536 x 384 35-37 us, of it 7.6
+// for the sum of 14 splits (33 MB of partials; the products alone are 13 us at the library's rate);
+// 262144 x 96 x 384 43-50;  400 x 256 x 256 7 (seven chunks in a row);  f32 65536 x 768 x 768 206-250
+// (310-375 TFLOP/s of the exact product, three times that of MFMA), 10007 x 299 x 203 19-22.
 // Tried and slower: a ring of three 32-token chunks (637 us against 612 at the time), two or three
 // chunks in flight in registers (the loads are not what it waits for; the first two asked for at once:
 // no change), a 128 x 128 tile a wave (four waves of 256 x 256: spills), 32-token chunks of the
@@ -122,7 +123,7 @@ constexpr int images(int columns) { return (columns + 127) / 128; }
 // branches drain the loads in flight).  Dwords: buffer loads, of rows that begin on a dword.  Halves:
 // buffer loads of the 20 B around a chunk of bf16, from the dword that its first value lies in, and a
 // shift by 0 or 16 bits on the way into LDS (40001 x 1030 x 1030 bf16, row pitch 1030 / 1031 values:
-// 130 / 142 us; by rows 238).
+// 130 / 139 us, by rows 238;  147456 x 1040 / 1039 x 2048 with db 683 / 745, without 676 / 727).
 enum Feed { kRows, kDwords, kHalves };
 
 // acc += h^T gY over the wave's TO x TI tiles of 32 x 32, chunk by chunk
