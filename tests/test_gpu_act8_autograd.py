@@ -151,3 +151,27 @@ def test_backbone_under_autocast():
         assert a.dtype == c.dtype == F32
         assert float((a.double() - c.double()).norm()) <= 0.05 * float(c.double().norm()) + 1e-12
     assert out[True][2] < out[False][2]
+
+
+@pytest.mark.parametrize("T", [50, 5000])
+def test_parameters_that_do_not_belong(T):
+    """A bias of another size or device, a weight of another device: what F.linear says to them (at
+    5000 tokens the token GEMM would read the bias itself)."""
+    import torch.nn.functional as F
+    from visionseg import ops
+    from visionseg.linear import linear_act8, linear_tokens, mlp_act8
+    x, w, b = _rand((T, 96), BF16, 1), _rand((288, 96), BF16, 2).requires_grad_(), _rand((288,), BF16, 3)
+    w2, b2 = _rand((96, 288), BF16, 4), _rand((96,), BF16, 5)
+    for wrong in (b[:7], b.cpu(), b.view(1, 288)[:, :5]):
+        with pytest.raises(RuntimeError):
+            F.linear(x, w, wrong)
+        for call in (lambda: linear_act8(x, w, wrong), lambda: mlp_act8(x, w, wrong, w2, b2),
+                     lambda: linear_tokens(x, w, wrong)):
+            with pytest.raises((RuntimeError, ValueError)):
+                call()
+        with pytest.raises((RuntimeError, ValueError)):
+            ops.token_gemm(x, w.detach(), wrong)
+    with pytest.raises(RuntimeError):
+        linear_act8(x, w.detach().cpu().requires_grad_(), b)
+    one = b[:1]                                              # one value for every output, as F.linear takes it
+    assert torch.equal(linear_act8(x, w, one), F.linear(x, w, one))

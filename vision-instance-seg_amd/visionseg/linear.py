@@ -140,7 +140,7 @@ def _forward_gemm(x, weight, bias):
     """x W^T + b inside _LinearFn.forward (grad mode is off there, so no _tgemm_ok)."""
     N, K = weight.shape
     if not (_TGEMM_FWD and x.is_cuda and x.dtype == weight.dtype == torch.bfloat16 and x.is_contiguous()
-            and (bias is None or bias.dtype == torch.bfloat16) and K % 8 == 0 and N % 8 == 0
+            and (bias is None or (bias.dtype == torch.bfloat16 and bias.shape == (N,))) and K % 8 == 0 and N % 8 == 0
             and x.numel() // K >= MIN_TOKENS and _use_token_gemm(x.numel() // K, N, K)):
         return F.linear(x, weight, bias)
     return ops.token_gemm(x.reshape(-1, K), weight, bias).view(*x.shape[:-1], N)
@@ -1093,9 +1093,9 @@ class _MlpAct8Fn(torch.autograd.Function):
 
 def _act8_ready(x, *params) -> bool:
     """Whether an act8 Function takes these: a device tensor that a gradient is wanted of, all
-    in one dtype of the kernels', no layer without inputs or outputs."""
+    in one dtype of the kernels' and on one device, no layer without inputs or outputs."""
     return (x.is_cuda and torch.is_grad_enabled() and x.dtype in (torch.float32, torch.bfloat16)
-            and all(p is None or (p.dtype == x.dtype and p.numel() > 0) for p in params))
+            and all(p is None or (p.dtype == x.dtype and p.device == x.device and p.numel() > 0) for p in params))
 
 
 def linear_act8(x, w, b=None):

@@ -2186,6 +2186,11 @@ def token_gemm(x, w, bias=None, gelu: bool = False, x_scales=None, w_scales=None
             or (gelu_pre is not None and (fp8 or gelu or bias is not None or N % 8 or gelu_pre.dtype != torch.bfloat16
                                           or gelu_pre.numel() != x.numel() // K * N)):
         raise ValueError(f"token_gemm: bad shapes x {tuple(x.shape)} w {tuple(w.shape)} fp8={fp8}")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16):
+        raise ValueError(f"token_gemm: bias {tuple(bias.shape)} {bias.dtype} is not bfloat16 [{N}]")
+    for t in (w, bias, x_scales, w_scales, gelu_pre):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"token_gemm: tensors on {x.device} and {t.device}")
     x2 = x.reshape(-1, K).contiguous()
     w = w.contiguous()
     # the kernel's 16-B LDS-DMA rows, 8-B bias and 4-B scale loads: a view with a storage
