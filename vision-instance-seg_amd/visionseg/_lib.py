@@ -7,6 +7,7 @@ something else.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -236,5 +237,15 @@ def ptr(t: torch.Tensor):
 
 
 def stream(t: torch.Tensor | None = None):
+    """The stream that work on t goes to.  t's device has to be the current one: another device's default
+    stream has the same handle, so the launch would run on the current device with pointers of the other."""
     dev = t.device if t is not None else None
+    if dev is not None and dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"visionseg: a tensor on {dev} while the current device is "
+                           f"cuda:{torch.cuda.current_device()} (enter torch.cuda.device({dev.index}) first)")
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)

@@ -1108,7 +1108,8 @@ def linear_act8(x, w, b=None):
             return linear_act8(x.to(dt), w.to(dt), None if b is None else b.to(dt))
     if not (_act8_ready(x, w, b) and w.requires_grad):
         return F.linear(x, w, b)
-    return _LinearAct8Fn.apply(x, w, b)
+    with L.on_device_of(x):
+        return _LinearAct8Fn.apply(x, w, b)
 
 
 def mlp_act8(x, w1, b1, w2, b2):
@@ -1122,7 +1123,8 @@ def mlp_act8(x, w1, b1, w2, b2):
     if not (_act8_ready(x, w1, b1, w2, b2)
             and any(p is not None and p.requires_grad for p in (x, w1, b1, w2, b2))):
         return F.linear(F.gelu(F.linear(x, w1, b1)), w2, b2)
-    return _MlpAct8Fn.apply(x, w1, b1, w2, b2)
+    with L.on_device_of(x):
+        return _MlpAct8Fn.apply(x, w1, b1, w2, b2)
 
 
 class TokenLinear(nn.Linear):
