@@ -71,3 +71,43 @@ def test_a_forward_without_a_backward_leaves_nothing(wt):
     for k in range(2000):
         batch.request(_w(3))
     assert not batch.pending
+
+
+def test_two_threads(wt):
+    """Forwards of one thread while another runs backwards: every get() is the transpose."""
+    import sys
+    import threading
+    batch, _, _ = wt
+    ws = [_w(k) for k in range(8)]
+    queue, errors, turns = [], [], 3000
+
+    def forwards():
+        for k in range(turns):
+            queue.append((batch.request(ws[k % 8]), ws[k % 8]))
+
+    def backwards():
+        done = 0
+        while done < turns and not errors:
+            if queue:
+                h, w = queue.pop(0)
+                if not torch.equal(batch.get(h), w.t()):
+                    errors.append(done)
+                done += 1
+
+    def guarded(f):
+        try:
+            f()
+        except Exception as e:
+            errors.append(e)
+
+    before = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=guarded, args=(f,)) for f in (forwards, backwards)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(60)
+    finally:
+        sys.setswitchinterval(before)
+    assert not errors, errors[:3]

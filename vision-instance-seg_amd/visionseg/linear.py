@@ -207,27 +207,31 @@ class _WeightTransposes:
     before their use, and a captured one runs at replays alone, when what was requested outside
     that capture has long been read or freed.  A request is held by its forward's autograd context
     and by nothing else, so a forward without a backward leaves none behind.  A backward that
-    finds itself elsewhere than its forward makes a copy of its own."""
+    finds itself elsewhere than its forward makes a copy of its own, and so does one whose request another
+    thread's work on the same tables has lost."""
 
     def __init__(self):
         self.live = {}                        # place -> its unwritten requests, oldest first
         self.count = 0
 
+    @staticmethod
+    def _handles(requests):
+        return [h for h in (r() for r in requests.valuerefs()) if h is not None]
+
     @property
     def pending(self):
-        return [h for hs in list(self.live.values()) for h in list(hs.values())]
+        return [h for hs in list(self.live.values()) for h in self._handles(hs)]
 
     def request(self, weight):
         h = _Transpose(weight, _place(weight))
         if h.place not in self.live:
-            self.live = {k: hs for k, hs in self.live.items() if len(hs)}
-            self.live[h.place] = weakref.WeakValueDictionary()
+            self.live = {k: hs for k, hs in list(self.live.items()) if len(hs)}
         self.count += 1
-        self.live[h.place][self.count] = h
+        self.live.setdefault(h.place, weakref.WeakValueDictionary())[self.count] = h
         return h
 
     def flush(self, place):
-        hs = list(self.live.pop(place, {}).values())
+        hs = self._handles(self.live.pop(place, weakref.WeakValueDictionary()))
         ops.transpose_batched([(h.weight.detach().contiguous(), h.out) for h in hs])
         for h in hs:
             h.done = True
