@@ -123,3 +123,51 @@ def test_gelu_f32_in_the_norm():
     want_y, want_gx = v * cdf, gy.double() * (cdf + v * torch.exp(-v * v / 2) / (2 * torch.pi) ** 0.5)
     assert float((y.detach().double() - want_y).norm() / want_y.norm()) <= 0.5 * U
     assert float((gx.double() - want_gx).norm() / want_gx.norm()) <= 0.9 * U
+
+
+def test_norm_and_gelu_beyond_32_bits():
+    """Tensors of more than 2^32 elements: rows there come out as they do in a tensor of their own."""
+    from visionseg import ops
+    C = 1000
+    rows = (1 << 32) // C + 9
+    at = torch.tensor([0, 1, (1 << 31) // C, (1 << 31) // C + 1, rows - 2, rows - 1], device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    some, grad = (torch.randn(6, C, generator=g, device=DEV).to(BF16) for _ in range(2))
+    w, b = (torch.rand(C, generator=g, device=DEV).to(BF16).requires_grad_() for _ in range(2))
+    few = some.clone().requires_grad_()
+    want = ops.layer_norm_act8(few, w, b), ops.gelu_act8(few)
+    want_gx = torch.autograd.grad(want[0], few, grad)[0], torch.autograd.grad(want[1], few, grad)[0]
+    x = torch.zeros(rows, C, device=DEV, dtype=BF16)
+    x[at] = some
+    x.requires_grad_()
+    gy = torch.zeros(rows, C, device=DEV, dtype=BF16)
+    gy[at] = grad
+    for k, op in enumerate((lambda: ops.layer_norm_act8(x, w, b), lambda: ops.gelu_act8(x))):
+        y = op()
+        assert torch.equal(y.detach()[at], want[k].detach())
+        gx = torch.autograd.grad(y, x, gy)[0]
+        assert torch.equal(gx[at], want_gx[k])
+        del y, gx
+    # a width without remainder (the kernels' flat form)
+    n = (1 << 32) // 1024 + 5
+    z = torch.zeros(n, 1024, device=DEV, dtype=BF16)
+    tail = torch.randn(3, 1024, generator=g, device=DEV).to(BF16)
+    z[-3:] = tail
+    assert torch.equal(ops.gelu_act8(z)[-3:], ops.gelu_act8(tail))
+
+
+def test_weight_gradient_of_more_than_32_bits():
+    """dW of more than 2^32 values."""
+    from visionseg import ops
+    T, N, K = 3, 66001, 66004
+    g = torch.Generator(device=DEV).manual_seed(5)
+    gy = torch.randint(-1, 2, (T, N), generator=g, device=DEV, dtype=torch.int8).to(BF16)
+    x = torch.randint(-15, 16, (T, K), generator=g, device=DEV, dtype=torch.int8).to(BF16)
+    q, scale = ops.act8_pack(x)
+    h = ops.act8_unpack(q, scale, K, F32).double()
+    dw, db = ops.act8_wgrad(gy, q, scale, K, BF16, bias=True)
+    ex.same(db, gy.double().sum(0), "db")
+    for r in (0, 1, (1 << 31) // K, (1 << 32) // K - 1, (1 << 32) // K, N - 1):
+        ex.same(dw[r], (gy[:, r].double()[:, None] * h).sum(0), f"row {r}")
+    cols = torch.tensor([0, 31, 32, K // 2, K - 1], device=DEV)
+    ex.same(dw[:, cols], gy.double().t().contiguous() @ h[:, cols].contiguous(), "columns")
