@@ -175,3 +175,32 @@ def test_parameters_that_do_not_belong(T):
         linear_act8(x, w.detach().cpu().requires_grad_(), b)
     one = b[:1]                                              # one value for every output, as F.linear takes it
     assert torch.equal(linear_act8(x, w, one), F.linear(x, w, one))
+
+
+@pytest.mark.parametrize("T", [300, 5000])
+@pytest.mark.parametrize("how", ["recomputed", "offloaded"])
+def test_saved_tensors_elsewhere(how, T):
+    """A block under torch's own activation checkpointing or offloading: the same results."""
+    from torch.utils.checkpoint import checkpoint
+    from visionseg import ops
+    from visionseg.linear import linear_act8, mlp_act8
+    C, H = 96, 384
+    ts = [_rand(s, BF16, k, 1.0 if k < 2 else 0.1).requires_grad_() for k, s in enumerate(
+        ((T, C), (T, C), (C,), (C,), (C, C), (C,), (H, C), (H,), (C, H), (C,)))]
+
+    def block(x, r, w, b, wq, bq, w1, b1, w2, b2):
+        s, y = ops.add_layer_norm_act8(x, r, w, b)
+        y = ops.gelu_act8(linear_act8(y, wq, bq))
+        return s + mlp_act8(ops.layer_norm_act8(y, w, b), w1, b1, w2, b2)
+
+    gy = _rand((T, C), BF16, 20)
+    want = block(*ts)
+    grads = torch.autograd.grad(want, ts, gy)
+    if how == "recomputed":
+        got = checkpoint(block, *ts, use_reentrant=False)
+        again = torch.autograd.grad(got, ts, gy)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            got = block(*ts)
+        again = torch.autograd.grad(got, ts, gy)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(again, grads))
