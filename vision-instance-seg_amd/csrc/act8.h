@@ -7,9 +7,10 @@
 // as q int8 [rows, P] (P = C rounded up to 32, zeros behind C) and scale uint8 [rows, P / 32] =
 // e + 127, and stands for q_i 2^e.  A power of two, so that the value is exact in bf16 (|q| < 128
 // is 7 bits) and a matrix product in bf16 sees exactly what the checkpoint stands for; an error
-// of at most 2^e / 2 <= max(a / 127, 2^-127) a value (e stops at -126).  A block that holds a magnitude above 127 2^121 (3.376e38,
-// where a rounded value can reach 2^128), an infinity or a NaN has scale 255 and q 0: 0 * 2^128 =
-// NaN, so a non-finite activation stays visible in the backward pass.
+// of at most 2^e / 2 <= max(a / 127, 2^-127) a value (e stops at -126).  A block that holds a
+// magnitude above 127 2^121 (3.376e38, where a rounded value can reach 2^128), an infinity or a NaN
+// has scale 255 and q 0: 0 * 2^128 = NaN, so a non-finite activation stays visible in the backward
+// pass.
 //
 // The unit of the kernels is a CHUNK of 8 consecutive features of a row: one 16-B load of bf16,
 // two of f32, one 8-B store of q.  A block is the 4 chunks of an aligned quad of lanes.
