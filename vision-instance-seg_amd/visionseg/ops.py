@@ -1543,13 +1543,14 @@ def activation(x, kind: str, gelu_sink=None):
 
 
 # ------------------------------------------------------------------ 8-bit activation checkpoints
-# What the backward pass reads of an activation, kept in one byte an element (csrc/act8.h): blocks
-# of 32 features share a power-of-two step 2^e, the smallest with which the block's largest
-# magnitude is at most 127 steps, so a value is off by at most 1 / 127 of its block's largest (but
-# for 2^-127 at the least: no step is finer than 2^-126) and is exact in bf16.  `q` int8 [..., P] (P = the features rounded up to 32, zeros behind them),
-# `scale` uint8 [..., P / 32] = e + 127; a block with an infinity or a NaN (or a magnitude
-# above 127 * 2^121) is kept as NaN (scale 255).  The forward results are not touched: only the
-# backward formulas are taken at the checkpointed values.
+# What the backward pass reads of an activation, kept in one byte an element (csrc/act8.h):
+# blocks of 32 features share a power-of-two step 2^e, the smallest with which the block's
+# largest magnitude is at most 127 steps, so a value is off by at most 1 / 127 of its block's
+# largest (but for 2^-127 at the least: no step is finer than 2^-126) and is exact in bf16.  `q`
+# int8 [..., P] (P = the features rounded up to 32, zeros behind them), `scale` uint8 [..., P /
+# 32] = e + 127; a block with an infinity or a NaN (or a magnitude above 127 * 2^121) is kept as
+# NaN (scale 255).  The forward results are not touched: only the backward formulas are taken at
+# the checkpointed values.
 _ACT8 = None
 
 
